@@ -415,6 +415,51 @@ int sfm_snippet_unpack(const unsigned char* seq, const float* K, int B, int H, i
                        float brightness, float col_r, float col_g, float col_b, int swap, float contrast, float* tgt,
                        float* src, float* K_ms, float* ws, void* stream);
 
+/* ---- group norm with an activation, and dropout (no counterpart in the reference, whose normaliser is batch norm) ------
+ * The batch-independent normaliser and the regulariser of the decoder's activations, channels last.  Tensors are fp32, bf16 or
+ * fp16 (dtype = SFM_F32 / SFM_BF16 / SFM_F16), aligned to their element; everything is computed in fp32 and a 16-bit result is
+ * rounded once, to nearest even; gamma, beta, the saved statistics and the parameter gradients are fp32.
+ *
+ * x [B, N, C]: B items of N rows (N = H*W) of C channels, G groups of C / G adjacent channels (G divides C; any C); rows are
+ * ld_x elements apart, items N * ld_x (a channel slice of a wider buffer: x = address of its first channel, ld_x >= C).
+ *   mean, var over the N * C / G values of an (item, group);  z = gamma (x - mean) / sqrt(var + eps) + beta
+ *   y = act(z)   or, with a mask,   y = keep ? act(z) * 65536 / (65536 - threshold) : 0
+ * save_mean, save_rstd [B, G] (both or neither; needed for the backward).
+ * Backward: dL/dy = gy[0] + ... + gy[n_gy - 1] (n_gy <= 3, each a channel slice with its own row stride ld_gy[k]; host arrays,
+ * read at call time) -> gx [B, N, C] dense (may be NULL), ggamma and gbeta [C] (both or neither), summed over items and rows.
+ * It reads x and not y, and takes the mask's arguments of the forward.
+ * ws: sfm_group_norm_workspace_floats(B, N, C, G, dtype, backward != 0) floats, 8-byte aligned, undefined between calls.
+ * Sums are joined in a fixed order: results are bitwise reproducible.
+ *
+ * The mask (threshold = 0: none) is a function of counters and never stored.  (seed, step): two 64-bit words at `rng` in device
+ * memory, read by the kernels (so a replayed graph follows them), or the two arguments if rng is NULL; of step the low 32 bits
+ * count.  An element of item b (counted from item0) at place e (= row * C + c; with per_channel e = c: whole channels of
+ * an item are dropped) takes the 16 bits (e % 8) of Philox 4x32 (7 rounds) of the counter (e / 8, item0 + b, step, layer) under
+ * the key `seed`, low half of a word first; it is kept if they are >= threshold, so the probability is threshold / 65536.
+ *
+ * sfm_dropout: y = keep ? x * 65536 / (65536 - threshold) : 0 for `items` dense items of item_elems elements (rows of C channels),
+ * and, applied to dL/dy, its own backward. */
+#define SFM_F32 0
+#define SFM_BF16 1
+#define SFM_F16 2
+#define SFM_ACT_NONE 0
+#define SFM_ACT_ELU 1
+#define SFM_ACT_RELU 2
+#define SFM_ACT_SILU 3
+long long sfm_group_norm_workspace_floats(long long B, long long N, int C, int G, int dtype, int backward);
+int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, const float* gamma, const float* beta, long long B,
+                           long long N, int C, int G, float eps, int act, const void* rng, unsigned long long seed,
+                           unsigned step, unsigned layer, unsigned item0, int threshold, int per_channel, void* y,
+                           long long ld_y, float* save_mean, float* save_rstd, float* ws, void* stream);
+int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, const void* const* gy, const long long* ld_gy, int n_gy,
+                           const float* gamma, const float* beta, const float* save_mean, const float* save_rstd,
+                           long long B, long long N, int C, int G, int act, const void* rng, unsigned long long seed,
+                           unsigned step, unsigned layer, unsigned item0, int threshold, int per_channel, void* gx,
+                           float* ggamma, float* gbeta, float* ws, void* stream);
+int sfm_dropout(const void* x, int dtype, long long items, long long item_elems, int C, const void* rng,
+                unsigned long long seed, unsigned step, unsigned layer, unsigned item0, int threshold, int per_channel,
+                void* y, void* stream);
+
 /* ---- measurement aid (no counterpart in the reference; used by bench.py only) -----------
  * When enabled, sfm_loss_forward / sfm_loss_backward bracket each of their launches with
  * HIP events on the caller's stream; sfm_prof_read adds the last step's elapsed ms per stage

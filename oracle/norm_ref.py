@@ -1,0 +1,83 @@
+"""Group norm with an activation and counter-based dropout from their definitions, in float64 on the CPU (NumPy): what the kernels
+of sfm_amd/csrc/group_norm.hip and dropout.hip are compared with.  No counterpart in the reference."""
+import numpy as np
+
+M0, M1, W0, W1 = 0xD2511F53, 0xCD9E8D57, 0x9E3779B9, 0xBB67AE85
+
+
+def philox(counter, key, rounds=7):
+    """Philox 4x32 (Salmon, Moraes, Dror, Shaw, SC 2011).  counter [..., 4], key [..., 2], 32-bit words -> [..., 4]"""
+    c = [np.asarray(counter[..., k], dtype=np.uint64) for k in range(4)]
+    k0, k1 = (np.asarray(key[..., k], dtype=np.uint64) for k in range(2))
+    lo = np.uint64(0xFFFFFFFF)
+    for _ in range(rounds):
+        a, b = c[0] * np.uint64(M0), c[2] * np.uint64(M1)
+        c = [(b >> np.uint64(32)) ^ c[1] ^ k0, b & lo, (a >> np.uint64(32)) ^ c[3] ^ k1, a & lo]
+        k0, k1 = (k0 + np.uint64(W0)) & lo, (k1 + np.uint64(W1)) & lo
+    return np.stack(c, axis=-1)
+
+
+def keep_mask(shape, threshold, seed, step=0, layer=0, per_channel=False, first_item=0):
+    """truth values of `shape` [B, ..., C]: what is kept"""
+    B, C = shape[0], shape[-1]
+    n = C if per_channel else int(np.prod(shape[1:]))
+    blocks = -(-n // 8)
+    ctr = np.zeros((B, blocks, 4), dtype=np.uint64)
+    ctr[..., 0] = np.arange(blocks)[None, :]
+    ctr[..., 1] = (first_item + np.arange(B))[:, None]
+    ctr[..., 2], ctr[..., 3] = step % 2 ** 32, layer
+    key = np.array([seed % 2 ** 32, (seed >> 32) % 2 ** 32], dtype=np.uint64)
+    w = philox(ctr, np.broadcast_to(key, (B, blocks, 2)))
+    u = np.stack([w & np.uint64(0xFFFF), w >> np.uint64(16)], axis=-1).reshape(B, blocks * 8)[:, :n]
+    keep = u >= threshold
+    return np.broadcast_to(keep.reshape((B,) + (1,) * (len(shape) - 2) + (C,)) if per_channel else keep.reshape(shape), shape)
+
+
+def act(z, kind):
+    if kind == "elu":
+        return np.where(z > 0, z, np.expm1(np.minimum(z, 0)))
+    if kind == "relu":
+        return np.maximum(z, 0)
+    if kind == "silu":
+        return z / (1 + np.exp(-z))
+    return z
+
+
+def act_grad(z, kind):
+    if kind == "elu":
+        return np.where(z > 0, 1.0, np.exp(np.minimum(z, 0)))
+    if kind == "relu":
+        return (z > 0).astype(np.float64)
+    if kind == "silu":
+        s = 1 / (1 + np.exp(-z))
+        return s * (1 + z * (1 - s))
+    return np.ones_like(z)
+
+
+def group_norm_act(x, gamma, beta, groups, eps, kind, gy=None, keep=None, threshold=0):
+    """x [B, ..., C] -> dict of y (and gx, ggamma, gbeta, and the sizes that error bounds are made of)"""
+    x, gamma, beta = (np.asarray(a, dtype=np.float64) for a in (x, gamma, beta))
+    B, C = x.shape[0], x.shape[-1]
+    v = x.reshape(B, -1, groups, C // groups)
+    ga, be = gamma.reshape(groups, -1), beta.reshape(groups, -1)
+    mean = v.mean(axis=(1, 3), keepdims=True)
+    rstd = 1 / np.sqrt(((v - mean) ** 2).mean(axis=(1, 3), keepdims=True) + eps)
+    xhat = (v - mean) * rstd
+    z = xhat * ga + be
+    scale = 1.0 if keep is None else 65536 / (65536 - threshold)
+    k = np.ones(v.shape) if keep is None else np.asarray(keep, dtype=np.float64).reshape(v.shape)
+    out = {"y": np.where(k > 0, scale * act(z, kind), 0.0).reshape(x.shape), "z": z.reshape(x.shape), "mean": mean.reshape(B, groups),
+           "rstd": rstd.reshape(B, groups)}
+    if gy is not None:
+        dz = np.where(k > 0, scale * np.asarray(gy, dtype=np.float64).reshape(v.shape), 0.0) * act_grad(z, kind)
+        dg = dz * ga
+        gx = rstd * (dg - dg.mean(axis=(1, 3), keepdims=True) - xhat * (dg * xhat).mean(axis=(1, 3), keepdims=True))
+        out.update(gx=gx.reshape(x.shape), ggamma=(dz * xhat).sum(axis=(0, 1)).reshape(C), gbeta=dz.sum(axis=(0, 1)).reshape(C),
+                   abs_ggamma=np.abs(dz * xhat).sum(axis=(0, 1)).reshape(C), abs_gbeta=np.abs(dz).sum(axis=(0, 1)).reshape(C),
+                   # the largest of each (item, group), broadcast: what an error of gx is measured against
+                   gx_size=np.broadcast_to(rstd * np.abs(dg).max(axis=(1, 3), keepdims=True)
+                                           * (1 + np.abs(xhat).max(axis=(1, 3), keepdims=True)) ** 2, v.shape).reshape(x.shape))
+    out["z_size"] = np.broadcast_to(1 + np.abs(ga).max() * (rstd * np.abs(v).max(axis=(1, 3), keepdims=True)
+                                                            + np.abs(xhat).max(axis=(1, 3), keepdims=True)),
+                                    v.shape).reshape(x.shape)
+    return out

@@ -20,6 +20,9 @@ _I = ctypes.c_int
 _L = ctypes.c_long
 _F = ctypes.c_float
 _LL = ctypes.c_longlong
+_ULL = ctypes.c_ulonglong
+_U = ctypes.c_uint
+_MASK = [_P, _ULL, _U, _U, _U, _I, _I]  # rng, seed, step, layer, item0, threshold, per_channel
 
 # name -> argtypes; must list every symbol of include/sfm_amd.h (checked by tests/test_abi.py)
 SIGNATURES = {
@@ -98,6 +101,10 @@ SIGNATURES = {
     "sfm_bn_elu_bwd_apply": [_P, _P, _P, _P, _P, _P, _P, _P, _LL, _LL, _I, _I, _P, _P],
     "sfm_snippet_workspace_floats": [_I, _I, _I, _I],
     "sfm_snippet_unpack": [_P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _F, _F, _I, _F, _P, _P, _P, _P, _P],
+    "sfm_group_norm_workspace_floats": [_LL, _LL, _I, _I, _I, _I],
+    "sfm_group_norm_act_fwd": [_P, _LL, _I, _P, _P, _LL, _LL, _I, _I, _F, _I, *_MASK, _P, _LL, _P, _P, _P, _P],
+    "sfm_group_norm_act_bwd": [_P, _LL, _I, _P, _P, _I, _P, _P, _P, _P, _LL, _LL, _I, _I, _I, *_MASK, _P, _P, _P, _P, _P],
+    "sfm_dropout": [_P, _I, _LL, _LL, _I, *_MASK, _P, _P],
     "sfm_prof_enable": [_I],
     "sfm_prof_stages": [],
     "sfm_prof_read": [_P],

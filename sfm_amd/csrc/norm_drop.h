@@ -1,0 +1,211 @@
+// Shared by the group norm and the dropout kernels: element types, vector loads, activations, the counter-based mask.
+#pragma once
+#include "sfm_device.h"
+#include "sfm_internal.h"
+#include <type_traits>
+
+namespace sfm {
+
+// ---- element types (SFM_F32 / SFM_BF16 / SFM_F16 of the C ABI).  Everything is computed in fp32; a 16-bit tensor is rounded
+// once, to nearest even, where it is stored.
+enum { kF32 = 0, kBF16 = 1, kF16 = 2 };
+template <int DT> struct ElemBytes { static constexpr int value = DT == kF32 ? 4 : 2; };
+
+template <int N> struct Words;  // N bytes as unsigned words, at any element alignment (global accesses need none wider)
+template <> struct Words<32> { typedef unsigned t __attribute__((ext_vector_type(8), aligned(4))); };
+template <> struct Words<16> { typedef unsigned t __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Words<8> { typedef unsigned t __attribute__((ext_vector_type(2), aligned(2))); };
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+struct __attribute__((packed, aligned(2))) PackedU32 { unsigned v; };
+
+// V consecutive elements in the registers they arrive in (V = 1: one element, zero-extended)
+template <int DT, int V> struct Raw { unsigned w[V * ElemBytes<DT>::value < 4 ? 1 : V * ElemBytes<DT>::value / 4]; };
+
+template <int DT, int V>
+__device__ __forceinline__ Raw<DT, V> load_raw(const void* __restrict__ base, long long elem) {
+  constexpr int kBytes = V * ElemBytes<DT>::value;
+  const char* p = static_cast<const char*>(base) + elem * ElemBytes<DT>::value;
+  Raw<DT, V> r;
+  if constexpr (kBytes == 2) r.w[0] = *reinterpret_cast<const unsigned short*>(p);
+  else if constexpr (kBytes == 4) r.w[0] = reinterpret_cast<const PackedU32*>(p)->v;
+  else if constexpr (kBytes == 32) {
+    const auto a = *reinterpret_cast<const Words<16>::t*>(p), b = *reinterpret_cast<const Words<16>::t*>(p + 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { r.w[k] = a[k]; r.w[4 + k] = b[k]; }
+  } else {
+    const auto a = *reinterpret_cast<const typename Words<kBytes>::t*>(p);
+#pragma unroll
+    for (int k = 0; k < kBytes / 4; ++k) r.w[k] = a[k];
+  }
+  return r;
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void unpack(const Raw<DT, V>& r, float (&f)[V]) {
+  if constexpr (DT == kF32) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = __uint_as_float(r.w[k]);
+  } else if constexpr (DT == kBF16) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = __uint_as_float(k & 1 ? r.w[k / 2] & 0xffff0000u : r.w[k / 2] << 16);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = (float)__builtin_bit_cast(_Float16, (unsigned short)(k & 1 ? r.w[k / 2] >> 16 : r.w[k / 2]));
+  }
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void store_vec(void* __restrict__ base, long long elem, const float (&f)[V]) {
+  constexpr int kBytes = V * ElemBytes<DT>::value;
+  char* p = static_cast<char*>(base) + elem * ElemBytes<DT>::value;
+  Raw<DT, V> r;
+  if constexpr (DT == kF32) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.w[k] = __float_as_uint(f[k]);
+  } else if constexpr (V == 1) {
+    if constexpr (DT == kBF16) r.w[0] = __builtin_bit_cast(unsigned short, (__bf16)f[0]);
+    else r.w[0] = __builtin_bit_cast(unsigned short, (_Float16)f[0]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const f32x2 v = {f[2 * k], f[2 * k + 1]};
+      if constexpr (DT == kBF16) r.w[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+      else r.w[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+    }
+  }
+  if constexpr (kBytes == 2) *reinterpret_cast<unsigned short*>(p) = (unsigned short)r.w[0];
+  else if constexpr (kBytes == 4) reinterpret_cast<PackedU32*>(p)->v = r.w[0];
+  else if constexpr (kBytes == 32) {
+    Words<16>::t a, b;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { a[k] = r.w[k]; b[k] = r.w[4 + k]; }
+    *reinterpret_cast<Words<16>::t*>(p) = a;
+    *reinterpret_cast<Words<16>::t*>(p + 16) = b;
+  } else {
+    typename Words<kBytes>::t a;
+#pragma unroll
+    for (int k = 0; k < kBytes / 4; ++k) a[k] = r.w[k];
+    *reinterpret_cast<typename Words<kBytes>::t*>(p) = a;
+  }
+}
+
+// ---- activations (SFM_ACT_* of the C ABI)
+enum { kActNone = 0, kActElu = 1, kActRelu = 2, kActSilu = 3 };
+constexpr float kLog2e = 1.44269504088896341f;
+
+// e^z by the hardware's base-2 exponential: relative error |z| 2^-24 from the rounded argument and an ulp of the instruction.
+// Results under 2^-126 become 0, which no activation below can tell from what they are.
+__device__ __forceinline__ float exp_fast(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
+
+// e^z - 1 for z <= 0.  e^z - 1 itself loses everything for small |z| (an absolute 2^-24 on a result of size |z|), so above -0.35
+// it is the Taylor polynomial to z^7 / 7! (what is left out is under 0.35^7 / 8! = 1.6e-8 of the result).
+__device__ __forceinline__ float expm1_neg(float z) {
+  float p = __builtin_fmaf(z, 1.0f / 5040.0f, 1.0f / 720.0f);
+  p = __builtin_fmaf(p, z, 1.0f / 120.0f);
+  p = __builtin_fmaf(p, z, 1.0f / 24.0f);
+  p = __builtin_fmaf(p, z, 1.0f / 6.0f);
+  p = __builtin_fmaf(p, z, 0.5f);
+  p = __builtin_fmaf(p * z, z, z);
+  return z > -0.35f ? p : exp_fast(z) - 1.0f;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-z)); }
+
+template <int V>
+__device__ __forceinline__ void act_fwd(float (&z)[V], int act) {  // act is uniform
+  if (act == kActElu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = z[k] > 0.0f ? z[k] : expm1_neg(z[k]);
+  } else if (act == kActRelu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = z[k] < 0.0f ? 0.0f : z[k];  // a NaN stays one
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = z[k] * sigmoid(z[k]);
+  }
+}
+
+// g[k] *= act'(z[k]); relu'(0) = 0, elu'(0) = 1
+template <int V>
+__device__ __forceinline__ void act_bwd(float (&g)[V], const float (&z)[V], int act) {
+  if (act == kActElu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) g[k] = z[k] > 0.0f ? g[k] : g[k] * exp_fast(z[k]);
+  } else if (act == kActRelu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) g[k] = z[k] > 0.0f ? g[k] : 0.0f;
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float s = sigmoid(z[k]);
+      g[k] *= s * __builtin_fmaf(z[k], 1.0f - s, 1.0f);
+    }
+  }
+}
+
+// ---- the dropout mask: a function of (seed, step, layer, item, place), never stored.
+// Philox 4x32 with seven rounds (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011; seven is the
+// fewest rounds that paper reports as passing BigCrush).  A call gives four words = eight 16-bit numbers, one per element: a
+// round is two 32 x 32 -> 64 bit products at a quarter of the ALU rate, so at 32 bits per element the generator and not memory
+// would bound a bf16 pass.  An element is kept where its number is >= threshold; what is kept is multiplied by
+// 65536 / (65536 - threshold), so the expectation is exact for the probability threshold / 65536 that is really used.
+struct Drop {
+  const unsigned long long* rng;  // device (seed, step), or NULL: the two below
+  unsigned long long seed;
+  unsigned step, layer, item0;
+  unsigned threshold;  // 0: nothing is dropped
+  float scale;
+  int per_channel;  // one number per (item, channel) instead of one per element
+};
+
+struct DropKey { unsigned k0, k1, step; };
+__device__ __forceinline__ DropKey drop_key(const Drop& d) {
+  const unsigned long long seed = d.rng ? d.rng[0] : d.seed;
+  return {(unsigned)seed, (unsigned)(seed >> 32), d.rng ? (unsigned)d.rng[1] : d.step};
+}
+
+__device__ __forceinline__ uint4 philox7(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned k0, unsigned k1) {
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
+    c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+    c1 = (unsigned)b;
+    c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+    c3 = (unsigned)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// keep bits of elements place .. place + V - 1 of an item, bit k for element k.  V is a power of two <= 8 that divides place: the
+// V elements lie in one block of eight.
+template <int V>
+__device__ __forceinline__ unsigned keep_bits(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
+  const uint4 r = philox7((unsigned)(place >> 3), item, key.step, d.layer, key.k0, key.k1);
+  const unsigned w[4] = {r.x, r.y, r.z, r.w};
+  unsigned all = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) all |= ((k & 1 ? w[k / 2] >> 16 : w[k / 2] & 0xffffu) >= d.threshold ? 1u : 0u) << k;
+  return V == 8 ? all : all >> (unsigned)(place & 7);
+}
+
+template <int V>
+__device__ __forceinline__ void drop_apply(float (&f)[V], unsigned keep, float scale) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) f[k] = (keep >> k) & 1 ? f[k] * scale : 0.0f;  // a dropped infinity or NaN is 0 as well
+}
+
+// the arguments of one mask as the C ABI passes them -> false if they are none
+static inline bool drop_args(const void* rng, unsigned long long seed, unsigned step, unsigned layer, unsigned item0,
+                             int threshold, int per_channel, Drop& d) {
+  if (threshold < 0 || threshold > 65535 || ((uintptr_t)rng & 7) != 0) return false;
+  d = Drop{static_cast<const unsigned long long*>(rng), seed, step, layer, item0, (unsigned)threshold,
+           65536.0f / (float)(65536 - threshold), per_channel != 0};
+  return true;
+}
+
+}  // namespace sfm
