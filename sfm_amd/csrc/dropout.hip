@@ -10,7 +10,7 @@ namespace {
 constexpr int kPer = 4;
 
 template <int DT>
-__global__ __launch_bounds__(kBlock) void dropout_kernel(const void* __restrict__ x, void* __restrict__ y, unsigned items,
+__global__ __launch_bounds__(kBlock) void dropout_kernel(const char* __restrict__ x, char* __restrict__ y, unsigned items,
                                                          unsigned long long n, unsigned blocks, unsigned C, Drop d) {
   const DropKey key = drop_key(d);
   const unsigned long long q0 = (unsigned long long)blockIdx.x * (kPer * kBlock);
@@ -23,7 +23,8 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const void* __restrict_
     const unsigned item = item0 + up;
     const unsigned long long first = (off - (unsigned long long)up * blocks) * 8;
     if (item >= items) continue;
-    const long long at = (long long)(item * n + first);
+    constexpr int kBytes = ElemBytes<DT>::value;
+    const long long at = (long long)(item * n + first) * kBytes;
     unsigned keep;
     if (d.per_channel) {  // the eight may start anywhere in a row of C channels and cross into the next
       keep = 0;
@@ -43,11 +44,11 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const void* __restrict_
       store_vec<DT, 8>(y, at, f);
     } else {
       for (unsigned e = 0; first + e < n; ++e) {
-        const auto r = load_raw<DT, 1>(x, at + e);
+        const auto r = load_raw<DT, 1>(x, at + e * kBytes);
         float f[1];
         unpack<DT, 1>(r, f);
         drop_apply<1>(f, keep >> e, d.scale);
-        store_vec<DT, 1>(y, at + e, f);
+        store_vec<DT, 1>(y, at + e * kBytes, f);
       }
     }
   }
@@ -75,7 +76,7 @@ extern "C" int sfm_dropout(const void* x, int dtype, long long items, long long 
   if (groups > 0x7fffffffll) return SFM_ERR_TOO_LARGE;
   const dim3 grid((unsigned)groups), block(kBlock);
   hipStream_t stream = (hipStream_t)stream_;
-#define SFM_DROP(DT) hipLaunchKernelGGL(dropout_kernel<DT>, grid, block, 0, stream, x, y, (unsigned)items, (unsigned long long)item_elems, (unsigned)blocks, (unsigned)C, d)
+#define SFM_DROP(DT) hipLaunchKernelGGL(dropout_kernel<DT>, grid, block, 0, stream, static_cast<const char*>(x), static_cast<char*>(y), (unsigned)items, (unsigned long long)item_elems, (unsigned)blocks, (unsigned)C, d)
   if (dtype == kF32) SFM_DROP(kF32);
   else if (dtype == kBF16) SFM_DROP(kBF16);
   else SFM_DROP(kF16);

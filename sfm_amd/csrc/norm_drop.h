@@ -2,6 +2,7 @@
 #pragma once
 #include "sfm_device.h"
 #include "sfm_internal.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace sfm {
@@ -24,10 +25,10 @@ struct __attribute__((packed, aligned(2))) PackedU32 { unsigned v; };
 // V consecutive elements in the registers they arrive in (V = 1: one element, zero-extended)
 template <int DT, int V> struct Raw { unsigned w[V * ElemBytes<DT>::value < 4 ? 1 : V * ElemBytes<DT>::value / 4]; };
 
-template <int DT, int V>
-__device__ __forceinline__ Raw<DT, V> load_raw(const void* __restrict__ base, long long elem) {
+template <int DT, int V, typename Offset>
+__device__ __forceinline__ Raw<DT, V> load_raw(const char* __restrict__ base, Offset bytes) {
   constexpr int kBytes = V * ElemBytes<DT>::value;
-  const char* p = static_cast<const char*>(base) + elem * ElemBytes<DT>::value;
+  const char* p = base + bytes;
   Raw<DT, V> r;
   if constexpr (kBytes == 2) r.w[0] = *reinterpret_cast<const unsigned short*>(p);
   else if constexpr (kBytes == 4) r.w[0] = reinterpret_cast<const PackedU32*>(p)->v;
@@ -57,10 +58,10 @@ __device__ __forceinline__ void unpack(const Raw<DT, V>& r, float (&f)[V]) {
   }
 }
 
-template <int DT, int V>
-__device__ __forceinline__ void store_vec(void* __restrict__ base, long long elem, const float (&f)[V]) {
+template <int DT, int V, typename Offset>
+__device__ __forceinline__ void store_vec(char* __restrict__ base, Offset bytes, const float (&f)[V]) {
   constexpr int kBytes = V * ElemBytes<DT>::value;
-  char* p = static_cast<char*>(base) + elem * ElemBytes<DT>::value;
+  char* p = base + bytes;
   Raw<DT, V> r;
   if constexpr (DT == kF32) {
 #pragma unroll
