@@ -24,6 +24,18 @@ namespace {
 #ifndef SFM_GN_U
 #define SFM_GN_U 4
 #endif
+#ifndef NT_STATS
+#define NT_STATS false
+#endif
+#ifndef NT_LAST
+#define NT_LAST false
+#endif
+#ifndef NT_STORE
+#define NT_STORE false
+#endif
+#ifndef NT_SUMS
+#define NT_SUMS false
+#endif
 constexpr int kTargetBlocks = SFM_GN_TARGET;  // eight workgroups of four waves per CU
 constexpr int kMaxChunks = 512;
 constexpr int kU = SFM_GN_U;                  // rows a thread has in flight
@@ -147,7 +159,7 @@ struct Rows {
   __device__ __forceinline__ bool valid(int t) const { return t < steps - 1 || (t == steps - 1 && ry < last); }
 };
 
-template <int DT, int V> struct Stream {
+template <int DT, int V, bool NT = false> struct Stream {
   static constexpr int kES = ElemBytes<DT>::value;
   const char* base;
   long long step;
@@ -159,13 +171,13 @@ template <int DT, int V> struct Stream {
     back = r.ry < r.last ? 0u : (unsigned)(r.ry * ld * kES);
   }
   __device__ __forceinline__ Raw<DT, V> load(const Rows& r, int t) const {  // t < r.steps, uniform
-    return load_raw<DT, V>(base + t * step, off - (t < r.steps - 1 ? 0u : back));
+    return load_raw<DT, V, NT>(base + t * step, off - (t < r.steps - 1 ? 0u : back));
   }
   __device__ __forceinline__ void batch(const Rows& r, int t0, Raw<DT, V> (&raw)[kU]) const {
     if (t0 + kU <= r.full) {
       const char* at = base + t0 * step;
 #pragma unroll
-      for (int u = 0; u < kU; ++u) { raw[u] = load_raw<DT, V>(at, off); at += step; }
+      for (int u = 0; u < kU; ++u) { raw[u] = load_raw<DT, V, NT>(at, off); at += step; }
     } else {
 #pragma unroll
       for (int u = 0; u < kU; ++u)
@@ -173,9 +185,9 @@ template <int DT, int V> struct Stream {
     }
   }
 };
-template <int DT, int V>
-__device__ __forceinline__ void store_row(const Stream<DT, V>& s, int t, const float (&f)[V]) {
-  store_vec<DT, V>(const_cast<char*>(s.base) + t * s.step, s.off, f);
+template <int DT, int V, bool NT>
+__device__ __forceinline__ void store_row(const Stream<DT, V, NT>& s, int t, const float (&f)[V]) {
+  store_vec<DT, V, NT>(const_cast<char*>(s.base) + t * s.step, s.off, f);
 }
 
 // Teams: the workgroup's threads, cut into teams of T lanes of one wave (T a power of two), one group each at a time.
@@ -207,7 +219,7 @@ __global__ __launch_bounds__(kBlock) void gn_stats_kernel(const void* __restrict
   const Where w = where(p, blockIdx.x);
   const Rows r(p, w);
   if (r.mine) {
-    const Stream<DT, V> xs(x, ldx, p, w, r);
+    const Stream<DT, V, NT_STATS> xs(x, ldx, p, w, r);
     float n = 0.0f, mean[A], m2[A];
 #pragma unroll
     for (int a = 0; a < A; ++a) { mean[a] = 0.0f; m2[a] = 0.0f; }
@@ -327,7 +339,8 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const void* __restrict
   __shared__ float2 stat[kBlock * A];
   const Where w = where(p, blockIdx.x);
   const Rows r(p, w);
-  const Stream<DT, V> xs(x, ldx, p, w, r), ys(y, ldy, p, w, r);
+  const Stream<DT, V, NT_LAST> xs(x, ldx, p, w, r);
+  const Stream<DT, V, NT_STORE> ys(y, ldy, p, w, r);
   Raw<DT, V> raw[kU];
   float sc[V], sh[V];
   const int c = w.c0 + r.vx * V;
@@ -409,7 +422,7 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restr
   const Where w = where(p, blockIdx.x);
   const Rows r(p, w);
   if (r.mine) {
-    const Stream<DT, V> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r);
+    const Stream<DT, V, NT_SUMS> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r);
     Raw<DT, V> xr[kU], gr[kU];
     xs.batch(r, 0, xr);
     gs.batch(r, 0, gr);
@@ -517,7 +530,8 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __rest
   }
   const Where w = where(p, blockIdx.x - param_blocks);
   const Rows r(p, w);
-  const Stream<DT, V> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r), os(gx, p.C, p, w, r);
+  const Stream<DT, V, NT_LAST> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r);
+  const Stream<DT, V, NT_STORE> os(gx, p.C, p, w, r);
   Raw<DT, V> xr[kU], gr[kU];
   const int c = w.c0 + r.vx * V;
   float mu[A], is[A], ga[V], be[V], c1[A], c2[A];

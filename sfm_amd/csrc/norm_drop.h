@@ -25,7 +25,11 @@ struct __attribute__((packed, aligned(2))) PackedU32 { unsigned v; };
 // V consecutive elements in the registers they arrive in (V = 1: one element, zero-extended)
 template <int DT, int V> struct Raw { unsigned w[V * ElemBytes<DT>::value < 4 ? 1 : V * ElemBytes<DT>::value / 4]; };
 
-template <int DT, int V, typename Offset>
+// (macros: a template parameter would drop the pointee's alignment)
+#define SFM_GET(NT, T, p) (NT ? __builtin_nontemporal_load(reinterpret_cast<const T*>(p)) : *reinterpret_cast<const T*>(p))
+#define SFM_PUT(NT, T, p, v) do { if (NT) __builtin_nontemporal_store(v, reinterpret_cast<T*>(p)); else *reinterpret_cast<T*>(p) = v; } while (0)
+
+template <int DT, int V, bool NT = false, typename Offset>
 __device__ __forceinline__ Raw<DT, V> load_raw(const char* __restrict__ base, Offset bytes) {
   constexpr int kBytes = V * ElemBytes<DT>::value;
   const char* p = base + bytes;
@@ -33,11 +37,11 @@ __device__ __forceinline__ Raw<DT, V> load_raw(const char* __restrict__ base, Of
   if constexpr (kBytes == 2) r.w[0] = *reinterpret_cast<const unsigned short*>(p);
   else if constexpr (kBytes == 4) r.w[0] = reinterpret_cast<const PackedU32*>(p)->v;
   else if constexpr (kBytes == 32) {
-    const auto a = *reinterpret_cast<const Words<16>::t*>(p), b = *reinterpret_cast<const Words<16>::t*>(p + 16);
+    const auto a = SFM_GET(NT, Words<16>::t, p), b = SFM_GET(NT, Words<16>::t, p + 16);
 #pragma unroll
     for (int k = 0; k < 4; ++k) { r.w[k] = a[k]; r.w[4 + k] = b[k]; }
   } else {
-    const auto a = *reinterpret_cast<const typename Words<kBytes>::t*>(p);
+    const auto a = SFM_GET(NT, typename Words<kBytes>::t, p);
 #pragma unroll
     for (int k = 0; k < kBytes / 4; ++k) r.w[k] = a[k];
   }
@@ -58,7 +62,7 @@ __device__ __forceinline__ void unpack(const Raw<DT, V>& r, float (&f)[V]) {
   }
 }
 
-template <int DT, int V, typename Offset>
+template <int DT, int V, bool NT = false, typename Offset>
 __device__ __forceinline__ void store_vec(char* __restrict__ base, Offset bytes, const float (&f)[V]) {
   constexpr int kBytes = V * ElemBytes<DT>::value;
   char* p = base + bytes;
@@ -83,13 +87,13 @@ __device__ __forceinline__ void store_vec(char* __restrict__ base, Offset bytes,
     Words<16>::t a, b;
 #pragma unroll
     for (int k = 0; k < 4; ++k) { a[k] = r.w[k]; b[k] = r.w[4 + k]; }
-    *reinterpret_cast<Words<16>::t*>(p) = a;
-    *reinterpret_cast<Words<16>::t*>(p + 16) = b;
+    SFM_PUT(NT, Words<16>::t, p, a);
+    SFM_PUT(NT, Words<16>::t, p + 16, b);
   } else {
     typename Words<kBytes>::t a;
 #pragma unroll
     for (int k = 0; k < kBytes / 4; ++k) a[k] = r.w[k];
-    *reinterpret_cast<typename Words<kBytes>::t*>(p) = a;
+    SFM_PUT(NT, typename Words<kBytes>::t, p, a);
   }
 }
 

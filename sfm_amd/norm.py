@@ -10,7 +10,6 @@ it is the same function for any batch size, in training and in serving, and need
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import Optional, Tuple, Union
@@ -19,19 +18,28 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr, stream_of
-from .aspp import BN_EPSILON, _grad_out
+from .aspp import BN_EPSILON, _grad_out, _sink_of
 from .utils import _check, _same_device
 
 Tensor = torch.Tensor
 GN_EPSILON = BN_EPSILON
 ACTIVATIONS = {None: 0, "none": 0, "elu": 1, "relu": 2, "silu": 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_HERE = contextlib.nullcontext()
+_autograd = None
 
 
-def _on(device):
-    """the device of the tensors as the current one (entering a device context costs more than asking)"""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _nodes():
+    """sfm_amd._autograd: the operators' autograd nodes (csrc/autograd.cpp)"""
+    global _autograd
+    if _autograd is None:
+        _lib.load()
+        try:
+            from . import _autograd as built
+        except ImportError as e:
+            raise ImportError("sfm_amd/_autograd.so is missing or was built for another torch - build it first (python -c 'import "
+                              "__graft_entry__ as g; g.build()' or make -C sfm_amd/csrc)") from e
+        _autograd = built
+    return _autograd
 
 
 def _check_activation(x, name: str) -> int:
@@ -45,34 +53,6 @@ def _check_activation(x, name: str) -> int:
     if x.dim() < 2:
         raise ValueError(f"{name} must be [B, ..., C] with at least two dimensions, got shape {tuple(x.shape)}")
     return dt
-
-
-def _rows(x: Tensor) -> Tuple[Tensor, int]:
-    """x [B, ..., C] as rows of C channels ld elements apart: itself if it is dense or a channel slice of a dense buffer, else a copy"""
-    if x.is_contiguous():
-        return x, x.shape[-1]
-    shape, stride = x.shape, x.stride()
-    if shape[-1] == 1 or stride[-1] == 1:
-        ld, want = None, None
-        for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
-            if n == 1:
-                continue
-            if ld is None:
-                ld = want = s
-            elif s != want:
-                break
-            want *= n
-        else:
-            if ld is None:
-                return x, shape[-1]
-            if ld >= shape[-1]:
-                return x, ld
-    return x.contiguous(), shape[-1]
-
-
-def _refuse_second_order(name: str) -> None:
-    if torch.is_grad_enabled():  # a backward runs with gradients on under create_graph=True alone: what it returns would lack its history
-        raise RuntimeError(f"{name} is differentiable once: its backward was called with create_graph=True")
 
 
 class DropoutMask:
@@ -120,10 +100,17 @@ class DropoutMask:
                            self.first_item)
 
     def _args(self):
-        return (ptr(self.rng), self.seed, self.step, self.layer, self.first_item, self.threshold, int(self.per_channel))
+        return (self.rng, self.seed, self.step, self.layer, self.first_item, self.threshold, self.per_channel)
 
 
-_NO_MASK = (None, 0, 0, 0, 0, 0, 0)
+_NO_MASK = (None, 0, 0, 0, 0, 0, False)
+
+
+def _ctypes_mask(mask):
+    if mask is None:
+        return _NO_MASK
+    rng, *rest = mask._args()
+    return (ptr(rng), *rest)
 
 
 def _check_mask(mask, x: Tensor) -> None:
@@ -136,76 +123,83 @@ def _check_mask(mask, x: Tensor) -> None:
 
 
 # ----------------------------------------------------------------------------- group norm
+class _Plan:
+    """what is known of a shape: sizes, and the floats of one buffer that holds the statistics (2 B G) and behind them the workspace
+    of either direction"""
+
+    __slots__ = ("B", "N", "C", "G", "dt", "stats", "fwd", "bwd")
+
+    def __init__(self, shape, dtype, groups):
+        C = shape[-1]
+        if groups < 1 or C < 1 or C % groups:
+            raise ValueError(f"groups must divide the {C} channels, got {groups}")
+        rows = 1
+        for n in shape[:-1]:
+            rows *= n
+        self.B, self.C, self.G, self.dt = shape[0], C, groups, _DTYPES[dtype]
+        self.N = rows // shape[0] if shape[0] else 0
+        self.stats = self.fwd = self.bwd = 0
+        if rows:
+            n = [_lib.load().sfm_group_norm_workspace_floats(self.B, self.N, C, groups, self.dt, back) for back in (0, 1)]
+            if min(n) < 0:
+                raise ValueError(f"unsupported group-norm shape {tuple(shape)} with {groups} groups (rc {min(n)})")
+            self.stats = 2 * self.B * groups                 # even: the workspace behind it stays aligned to 8 bytes
+            self.fwd, self.bwd = n
+
+
 @functools.lru_cache(maxsize=1024)
-def _workspace_floats(B, N, C, G, dt, backward) -> int:
-    n = _lib.load().sfm_group_norm_workspace_floats(B, N, C, G, dt, backward)
-    if n < 0:
-        raise ValueError(f"unsupported group-norm shape B={B} N={N} C={C} G={G} (rc {n})")
-    return n
+def _plan(shape, dtype, groups) -> _Plan:
+    return _Plan(shape, dtype, groups)
 
 
-def _workspace(B, N, C, G, dt, backward, device) -> Tensor:
-    return torch.empty((_workspace_floats(B, N, C, G, dt, backward) + 1) // 2, dtype=torch.float64, device=device)
+def _raw_gn(plan, x, ld_x, gamma, beta, epsilon, act, mask, y, ld_y, keep):
+    """-> the buffer of statistics and workspace (keep: large enough for the backward, which takes it).  y: a tensor of its own or
+    a channel slice (row stride ld_y)"""
+    p = plan
+    buf = torch.empty(p.stats + max(p.fwd, p.bwd) if keep else p.fwd, dtype=torch.float32, device=x.device)
+    at = buf.data_ptr()
+    call("sfm_group_norm_act_fwd", ptr(x), ld_x, p.dt, ptr(gamma), ptr(beta), p.B, p.N, p.C, p.G, epsilon, act, *_ctypes_mask(mask),
+         ptr(y), ld_y, at if keep else None, at + 2 * p.stats if keep else None, at + 4 * p.stats if keep else at, stream_of(x))
+    return buf
 
 
-def _raw_gn(x, ld_x, gamma, beta, groups, epsilon, act, mask, y, ld_y, stats):
-    """-> (mean, rstd) [B, G] if stats; y: a tensor of its own or a channel slice (row stride ld_y)"""
-    B, C = x.shape[0], x.shape[-1]
-    N = x.numel() // (B * C)
-    dt = _DTYPES[x.dtype]
-    ws = _workspace(B, N, C, groups, dt, 0, x.device)
-    mean = rstd = None
-    if stats:
-        mean = torch.empty(B, groups, dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-    call("sfm_group_norm_act_fwd", ptr(x), ld_x, dt, ptr(gamma), ptr(beta), B, N, C, groups, epsilon, act,
-         *(_NO_MASK if mask is None else mask._args()), ptr(y), ld_y, ptr(mean), ptr(rstd), ptr(ws), stream_of(x))
-    return mean, rstd
-
-
-def _raw_gn_bwd(x, ld_x, srcs, gamma, beta, stats, groups, act, mask, need_x=True, need_params=True):
+def _raw_gn_bwd(plan, x, ld_x, srcs, gamma, beta, buf, act, mask, need_x=True, need_params=True):
     """srcs: [(tensor whose data pointer is the slice's first channel at row 0, row stride)], summed while loading"""
-    B, C = x.shape[0], x.shape[-1]
-    N = x.numel() // (B * C)
-    dt = _DTYPES[x.dtype]
-    ws = _workspace(B, N, C, groups, dt, 1, x.device)
+    p, n = plan, len(srcs)
     gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
     gg, gb = (_grad_out(gamma), _grad_out(beta)) if need_params else (None, None)
-    n = len(srcs)
-    gy = (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in srcs])
-    ld = (ctypes.c_longlong * n)(*[int(l) for _, l in srcs])
-    call("sfm_group_norm_act_bwd", ptr(x), ld_x, dt, gy, ld, n, ptr(gamma), ptr(beta), ptr(stats[0]), ptr(stats[1]), B, N, C,
-         groups, act, *(_NO_MASK if mask is None else mask._args()), ptr(gx), ptr(gg), ptr(gb), ptr(ws), stream_of(x))
+    at = buf.data_ptr()
+    call("sfm_group_norm_act_bwd", ptr(x), ld_x, p.dt, (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in srcs]),
+         (ctypes.c_longlong * n)(*[ld for _, ld in srcs]), n, ptr(gamma), ptr(beta), at, at + 2 * p.stats, p.B, p.N, p.C, p.G, act,
+         *_ctypes_mask(mask), ptr(gx), ptr(gg), ptr(gb), at + 4 * p.stats, stream_of(x))
     return gx, gg, gb
 
 
-class _GroupNormAct(torch.autograd.Function):
+class _GroupNormActInBuckets(torch.autograd.Function):
+    """the same node as sfm_amd._autograd's, in Python, for parameters whose gradients are born inside a ``GradBuckets``"""
+
     @staticmethod
-    def forward(ctx, x, gamma, beta, groups, epsilon, act, mask):
-        with _on(x.device):
+    def forward(ctx, x, gamma, beta, plan, epsilon, act, mask):
+        x = x.contiguous()
+        with torch.cuda.device(x.device):
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            if x.numel() == 0:
-                mean = rstd = None
-            else:
-                rows, ld = _rows(x)
-                mean, rstd = _raw_gn(rows, ld, gamma, beta, groups, epsilon, act, mask, y, x.shape[-1], True)
-        ctx.save_for_backward(x, gamma, beta, mean, rstd, None if mask is None else mask.rng)
-        ctx.cfg = (groups, act, mask)
+            buf = _raw_gn(plan, x, plan.C, gamma, beta, epsilon, act, mask, y, plan.C, True) if plan.fwd else None
+        ctx.save_for_backward(x, gamma, beta, buf, None if mask is None else mask.rng)
+        ctx.cfg = (plan, act, mask)
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        _refuse_second_order("group_norm_act")
-        x, gamma, beta, mean, rstd, _ = ctx.saved_tensors  # (unpacking checks that the mask's rng is what the forward read)
-        groups, act, mask = ctx.cfg
-        need_x, need_params = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        with _on(x.device):
-            if x.numel() == 0:
-                gx, gg, gb = torch.zeros_like(x), torch.zeros_like(gamma), torch.zeros_like(beta)
-            else:
-                rows, ld = _rows(x)
-                gx, gg, gb = _raw_gn_bwd(rows, ld, [_rows(gy)], gamma, beta, (mean, rstd), groups, act, mask, need_x, need_params)
-        return gx, gg, gb, None, None, None, None
+        if torch.is_grad_enabled():  # a backward runs with gradients on under create_graph=True alone
+            raise RuntimeError("group_norm_act is differentiable once: its backward was called with create_graph=True")
+        x, gamma, beta, buf, _ = ctx.saved_tensors  # (unpacking checks that the mask's rng is what the forward read)
+        plan, act, mask = ctx.cfg
+        if buf is None:
+            return torch.zeros_like(x), torch.zeros_like(gamma), torch.zeros_like(beta), None, None, None, None
+        need_x, need_g, need_b = ctx.needs_input_grad[:3]
+        with torch.cuda.device(x.device):
+            return (*_raw_gn_bwd(plan, x, plan.C, ((gy.contiguous(), plan.C),), gamma, beta, buf, act, mask, need_x, need_g or need_b),
+                    None, None, None, None)
 
 
 def group_norm_act(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon: float = GN_EPSILON,
@@ -216,14 +210,18 @@ def group_norm_act(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon:
     adjacent channels the mean and the population variance over all rows, z = gamma (x - mean) / sqrt(var + epsilon) + beta, the
     activation ("elu", "relu", "silu" or None), and, with a ``DropoutMask``, the mask.  Statistics and parameter gradients are
     fp32 for every type.  Differentiable once, in x, gamma and beta; the backward reads x and forms z and the mask again."""
-    dt = _check_activation(x, "x")
-    C = x.shape[-1]
-    gamma = _check(gamma, "gamma", 1, C)
-    beta = _check(beta, "beta", 1, C)
-    _same_device(x, gamma, beta)
-    groups, epsilon = int(groups), float(epsilon)
-    if groups < 1 or C < 1 or C % groups:
-        raise ValueError(f"groups must divide the {C} channels, got {groups}")
+    _check_activation(x, "x")
+    shape, device = x.shape, x.device
+    C = shape[-1]
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        if not (isinstance(t, Tensor) and t.dtype is torch.float32 and t.dim() == 1 and t.shape[0] == C and t.device == device):
+            _check(t, name, 1, C)
+            _same_device(x, t)
+    if not gamma.is_contiguous():
+        gamma = gamma.contiguous()
+    if not beta.is_contiguous():
+        beta = beta.contiguous()
+    epsilon = float(epsilon)
     if not 0.0 < epsilon < float("inf"):
         raise ValueError(f"epsilon must be positive and finite, got {epsilon}")
     act = ACTIVATIONS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
@@ -233,51 +231,19 @@ def group_norm_act(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon:
         _check_mask(dropout, x)
         if dropout.threshold == 0:
             dropout = None
-    if x.numel():
-        _workspace_floats(x.shape[0], x.numel() // (x.shape[0] * C), C, groups, dt, 0)
-    if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
-        return _GroupNormAct.apply(x, gamma, beta, groups, epsilon, act, dropout)
-    with _on(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if x.numel():
-            rows, ld = _rows(x.detach())
-            _raw_gn(rows, ld, gamma, beta, groups, epsilon, act, dropout, y, C, False)
-    return y
+    groups = int(groups)
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError(f"groups must divide the {C} channels, got {groups}")
+    if torch.is_grad_enabled() and (_sink_of(gamma) is not None or _sink_of(beta) is not None):
+        return _GroupNormActInBuckets.apply(x, gamma, beta, _plan(shape, x.dtype, groups), epsilon, act, dropout)
+    return _nodes().group_norm_act(x, gamma, beta, groups, epsilon, act, *(_NO_MASK if dropout is None else dropout._args()))
 
 
 # ----------------------------------------------------------------------------- dropout
-def _raw_dropout(x, mask):
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    if x.numel():
-        call("sfm_dropout", ptr(x), _DTYPES[x.dtype], x.shape[0], x.numel() // x.shape[0], x.shape[-1], *mask._args(), ptr(y),
-             stream_of(x))
-    return y
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, mask):
-        ctx.save_for_backward(mask.rng)
-        ctx.mask = mask
-        with _on(x.device):
-            return _raw_dropout(x, mask)
-
-    @staticmethod
-    def backward(ctx, gy):
-        _refuse_second_order("dropout")
-        ctx.saved_tensors  # (checks that the mask's rng is what the forward read)
-        with _on(gy.device):
-            return _raw_dropout(gy, ctx.mask), None
-
-
 def dropout(x: Tensor, mask: DropoutMask) -> Tensor:
     """``x`` [B, ..., C] (fp32, bf16 or fp16) with the elements, or the channels, that ``mask`` drops set to 0 and the others
     multiplied by 1 / (1 - mask.probability).  What is dropped is 0 even where x is infinite or NaN.  Differentiable once: the backward
     draws the same mask again, nothing is kept for it."""
     _check_activation(x, "x")
     _check_mask(mask, x)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, mask)
-    with _on(x.device):
-        return _raw_dropout(x.detach(), mask)
+    return _nodes().dropout(x, *mask._args())
