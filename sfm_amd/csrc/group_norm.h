@@ -1,0 +1,253 @@
+// Group norm with an activation (and a dropout mask), channels last: x [B, N, C] (N rows of an item), G groups of cpg = C / G
+// adjacent channels, m = N cpg values per (item, group).
+//
+//   mean = sum x / m     var = sum (x - mean)^2 / m     r = rsqrt(var + eps)
+//   xhat = (x - mean) r     z = gamma xhat + beta     y = k s act(z)          k, s: keep bit and factor of the mask (norm_drop.h)
+//
+//   dz = gy k s act'(z)     gbeta = sum_{b,n} dz     ggamma = sum_{b,n} dz xhat
+//   gx = r (gamma dz - c1 - xhat c2)     c1 = sum_group gamma dz / m     c2 = sum_group gamma dz xhat / m
+//
+// Two launches per direction: partial sums of chunks of rows, then a pass that joins the partials of its groups and applies.  z is
+// formed again from x in the backward, so y is not kept.  No atomics: partials are joined in a fixed order.
+//
+// Statistics: a thread takes the mean of a few rows in registers, then the squared deviations from it, and joins such
+// batches by Chan's update of (count, mean, M2); so does everything above it.  Nothing is a difference of large sums, whatever
+// the mean of a group is against its deviation.
+//
+// This file: what both directions share.
+#pragma once
+#include "norm_drop.h"
+
+namespace sfm {
+namespace {
+
+
+constexpr int kTargetBlocks = 1024;  // four workgroups of four waves per CU: all of a launch is resident (2048 was two rounds of most kernels)
+constexpr int kMaxChunks = 512;
+constexpr int kU = 4;                  // rows a thread has in flight
+
+// How an item is cut: channels into slabs (whole groups, or an even part of one wide group), rows into chunks.
+struct GnPlan {
+  long long N;
+  int C, G, cpg;
+  int V;                 // elements per thread and row
+  int cs;                // channels of a slab (the last one of a group or of the row may have fewer)
+  int slabs;             // slabs of a row
+  int groups_per_slab;   // >= 1; 1 where a group has parts
+  int parts;             // slabs of a group (1 where a slab holds whole groups)
+  int lanes;             // cs / V
+  int row_lanes;         // kBlock / lanes: rows a workgroup takes at once
+  int chunks;
+  int rows_per_chunk;
+  int P;                 // partials of a group: chunks * parts
+};
+
+static inline int gcd_int(int a, int b) {
+  while (b) { const int t = a % b; a = b; b = t; }
+  return a;
+}
+
+// (the arguments have been checked; false: an item is too large)
+static bool gn_plan(long long B, long long N, int C, int G, int es, GnPlan& p) {
+  p.N = N; p.C = C; p.G = G; p.cpg = C / G;
+  p.V = 16 / es;
+  while (C % p.V) p.V /= 2;
+  // a slab of whole groups is a multiple of lcm(cpg, V); where that is too wide for a workgroup and V does not divide a group
+  // either (a part of a group has to start at a multiple of V), a smaller V does
+  for (;; p.V /= 2) {
+    if (p.cpg % p.V == 0) break;
+    if (p.cpg / gcd_int(p.cpg, p.V) <= kBlock) break;
+  }
+  const int unit_groups = p.V / gcd_int(p.cpg, p.V);                      // groups of the smallest slab
+  const long long unit = (long long)p.cpg * unit_groups;
+  if (unit / p.V <= kBlock) {
+    long long k = 1;  // at least 128 bytes of a row, so that a slab's lines are its own
+    while (k * unit * es < 128 && k * unit < C) ++k;
+    while (k > 1 && k * unit / p.V > kBlock) --k;
+    p.groups_per_slab = k * unit_groups < G ? (int)k * unit_groups : G;
+    p.cs = p.groups_per_slab * p.cpg;
+    p.parts = 1;
+    p.slabs = (G + p.groups_per_slab - 1) / p.groups_per_slab;
+  } else {
+    const int vecs = p.cpg / p.V;
+    p.groups_per_slab = 1;
+    p.parts = (vecs + kBlock - 1) / kBlock;
+    p.cs = (vecs + p.parts - 1) / p.parts * p.V;
+    p.parts = (p.cpg + p.cs - 1) / p.cs;
+    if ((long long)G * p.parts > 0x7fffffffll) return false;
+    p.slabs = G * p.parts;
+  }
+  p.lanes = p.cs / p.V;
+  p.row_lanes = kBlock / p.lanes;
+  const long long per = (long long)B * p.slabs, step = (long long)kU * p.row_lanes;
+  long long chunks = (kTargetBlocks + per - 1) / per;
+  const long long most = (N + step - 1) / step;  // a full batch per thread at least
+  if (chunks > most) chunks = most;
+  if (chunks > kMaxChunks) chunks = kMaxChunks;
+  if (chunks < 1) chunks = 1;
+  long long rows = (N + chunks - 1) / chunks;
+  if (rows > step) rows = (rows + step - 1) / step * step;  // whole batches in all chunks but the last
+  if (rows > 0x7fffffffll) return false;
+  p.rows_per_chunk = (int)rows;
+  p.chunks = (int)((N + rows - 1) / rows);
+  p.P = p.chunks * p.parts;
+  return true;
+}
+
+// ---- what a workgroup works on
+struct Where {
+  int b, slab, chunk, part;
+  int c0, cc, g0, ng;  // first channel and channels of the slab, first group and groups of it
+  long long r0;        // first row, in the item
+  int rows;
+};
+__device__ __forceinline__ Where where(const GnPlan& p, unsigned bid) {
+  Where w;
+  w.chunk = bid % (unsigned)p.chunks;
+  bid /= (unsigned)p.chunks;
+  w.slab = bid % (unsigned)p.slabs;
+  w.b = bid / (unsigned)p.slabs;
+  if (p.parts == 1) {
+    w.part = 0;
+    w.g0 = w.slab * p.groups_per_slab;
+    w.ng = min(p.groups_per_slab, p.G - w.g0);
+    w.c0 = w.g0 * p.cpg;
+    w.cc = w.ng * p.cpg;
+  } else {
+    w.g0 = w.slab / p.parts;
+    w.part = w.slab % p.parts;
+    w.ng = 1;
+    w.c0 = w.g0 * p.cpg + w.part * p.cs;
+    w.cc = min(p.cs, p.cpg - w.part * p.cs);
+  }
+  w.r0 = (long long)w.chunk * p.rows_per_chunk;
+  w.rows = (int)min((long long)p.rows_per_chunk, p.N - w.r0);
+  return w;
+}
+
+// The rows of a thread: vector vx of the slab in rows ry, ry + row_lanes, ... of the chunk, one per step, in batches of kU steps.  The
+// address of a load is a uniform pointer that moves with the step and a 32-bit offset of the thread (gn_setup keeps row_lanes rows
+// under 2^31 bytes).
+struct Rows {
+  int vx, ry;
+  bool mine;     // this thread has a vector at all
+  int steps;     // of the chunk
+  int last;      // rows of its last step (1 .. row_lanes)
+  int full;      // steps in which every row lane has a row
+  __device__ __forceinline__ Rows(const GnPlan& p, const Where& w) {
+    vx = threadIdx.x % (unsigned)p.lanes;
+    ry = threadIdx.x / (unsigned)p.lanes;
+    mine = ry < p.row_lanes && vx * p.V < w.cc;
+    steps = (w.rows + p.row_lanes - 1) / p.row_lanes;
+    last = w.rows - (steps - 1) * p.row_lanes;
+    full = last == p.row_lanes ? steps : steps - 1;
+  }
+  __device__ __forceinline__ bool valid(int t) const { return t < steps - 1 || (t == steps - 1 && ry < last); }
+};
+
+// NT: nontemporal, for tensors that no cache holds until they are read again (far(), below)
+template <int DT, int V, bool NT = false> struct Stream {
+  static constexpr int kES = ElemBytes<DT>::value;
+  const char* base;
+  long long step;
+  unsigned off, back;  // back: in the last step a row lane without a row reads row lane 0's
+  __device__ __forceinline__ Stream(const void* p, long long ld, const GnPlan& pl, const Where& w, const Rows& r) {
+    base = static_cast<const char*>(p) + (((long long)w.b * pl.N + w.r0) * ld + w.c0) * kES;
+    step = (long long)pl.row_lanes * ld * kES;
+    off = (unsigned)((r.ry * ld + r.vx * V) * kES);
+    back = r.ry < r.last ? 0u : (unsigned)(r.ry * ld * kES);
+  }
+  __device__ __forceinline__ Raw<DT, V> load(const Rows& r, int t) const {  // t < r.steps, uniform
+    return load_raw<DT, V, NT>(base + t * step, off - (t < r.steps - 1 ? 0u : back));
+  }
+  __device__ __forceinline__ void batch(const Rows& r, int t0, Raw<DT, V> (&raw)[kU]) const {
+    if (t0 + kU <= r.full) {
+      const char* at = base + t0 * step;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) { raw[u] = load_raw<DT, V, NT>(at, off); at += step; }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (t0 + u < r.steps) raw[u] = load(r, t0 + u);
+    }
+  }
+};
+template <int DT, int V, bool NT>
+__device__ __forceinline__ void store_row(const Stream<DT, V, NT>& s, int t, const float (&f)[V]) {
+  store_vec<DT, V, NT>(const_cast<char*>(s.base) + t * s.step, s.off, f);
+}
+
+// Teams: the workgroup's threads, cut into teams of T lanes of one wave (T a power of two), one group each at a time.
+struct Team { int T, id, lane, count; };
+__device__ __forceinline__ Team team_of(int ng) {
+  int T = 64;
+  while (T > 1 && kBlock / T < ng) T >>= 1;
+  return {T, (int)threadIdx.x / T, (int)threadIdx.x & (T - 1), kBlock / T};
+}
+template <typename F> __device__ __forceinline__ F team_sum(F v, int T) {
+  for (int o = T >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// values that partial q of a group covers
+__device__ __forceinline__ double part_count(const GnPlan& p, int q) {
+  const int chunk = p.parts == 1 ? q : q / p.parts, part = q - chunk * p.parts;
+  const int rows = chunk == p.chunks - 1 ? (int)(p.N - (long long)chunk * p.rows_per_chunk) : p.rows_per_chunk;
+  return (double)rows * (p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
+}
+
+// dispatch on the type, the vector width and whether a vector lies in one group: fn(DT, V, ONE) as integral constants
+template <typename F> static void by_type(int dtype, const GnPlan& p, F&& fn) {
+  using std::integral_constant;
+  const bool one = p.cpg % p.V == 0;
+  auto width = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    auto go = [&](auto v) {
+      if (one) fn(dt, v, std::true_type{});
+      else if constexpr (decltype(v)::value > 1) fn(dt, v, std::false_type{});
+    };
+    if constexpr (DT != kF32) { if (p.V == 8) return go(integral_constant<int, 8>{}); }
+    if (p.V == 4) return go(integral_constant<int, 4>{});
+    if (p.V == 2) return go(integral_constant<int, 2>{});
+    go(integral_constant<int, 1>{});
+  };
+  if (dtype == kF32) return width(integral_constant<int, kF32>{});
+  if (dtype == kBF16) return width(integral_constant<int, kBF16>{});
+  width(integral_constant<int, kF16>{});
+}
+
+// fn(DROP, FAR): nontemporal accesses come in the full width alone
+template <int DT, int V, typename F> static void by_use(bool drop, bool away, F&& fn) {
+  if constexpr (V * ElemBytes<DT>::value == 16) {
+    if (away && drop) return fn(std::true_type{}, std::true_type{});
+    if (away) return fn(std::false_type{}, std::true_type{});
+  }
+  if (drop) fn(std::true_type{}, std::false_type{});
+  else fn(std::false_type{}, std::false_type{});
+}
+
+// The last pass over tensors that together pass the memory-side cache (256 MB) reads and writes nontemporally: nothing of them would be found
+// there again.  1024x2048x32 bf16 serve 650 -> 605 us, train 863 -> 778; under it a reader of the result may still find it, and
+// the pass itself gains little (concat4 of the 128x416 decoder, 54 MB a tensor: 87.1 -> 84.5 us for four passes).
+static inline bool far(long long bytes) { return bytes > (256ll << 20); }
+
+// rows of C elements of es bytes, ld elements apart
+static bool rows_ok(const void* q, long long ld, int C, int es) { return q && ld >= C && ((uintptr_t)q & (es - 1)) == 0; }
+
+// ld: the widest row stride of the call
+static int gn_setup(long long B, long long N, int C, int G, int dtype, long long ld, GnPlan& p, unsigned& grid) {
+  if (dtype < kF32 || dtype > kF16 || B < 1 || N < 1 || C < 1 || G < 1 || C % G || ld < C) return SFM_ERR_ARG;
+  const int es = dtype == kF32 ? 4 : 2;
+  // items are counted in 32 bits, workgroups in 31, elements in 60 with room for strides; the rows that a workgroup takes at once
+  // lie within 31 bits of bytes of each other
+  if (B > 0x7fffffffll || (__int128)B * N > ((__int128)1 << 40) || ld > 0x7fffffffll / es || !gn_plan(B, N, C, G, es, p))
+    return SFM_ERR_TOO_LARGE;
+  p.row_lanes = (int)std::min<long long>(p.row_lanes, 0x7fffffffll / (ld * es));
+  const __int128 blocks = (__int128)B * p.slabs * p.chunks;
+  if (blocks + C > 0x7fffffffll) return SFM_ERR_TOO_LARGE;
+  grid = (unsigned)blocks;
+  return SFM_OK;
+}
+
+}  // namespace
+}  // namespace sfm

@@ -1,0 +1,262 @@
+// Group norm with an activation: the backward (group_norm.h has the mathematics and the plan).
+#include "group_norm.h"
+
+namespace sfm {
+namespace {
+
+// dL/dy: the sum of up to three tensors, each a channel slice with its own row stride (what an activation's several readers
+// hand back in a decoder level without concats)
+struct GySrc {
+  const void* p[3];
+  long long ld[3];
+  int n;
+};
+template <int DT, int V>
+__device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, const Where& w, const Rows& r, int t, float (&g)[V]) {
+  for (int k = 1; k < s.n; ++k) {  // uniform
+    const Stream<DT, V> more(s.p[k], s.ld[k], p, w, r);
+    float f[V];
+    unpack<DT, V>(more.load(r, t), f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) g[e] += f[e];
+  }
+}
+
+// ---- backward, first launch: per_group [B][G][P] (sum gamma dz, sum gamma dz xhat), per_channel [C][B][chunks] (sum dz, sum dz xhat)
+template <int DT, int V, bool ONE, bool DROP>
+__global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+                                                             const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                             const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                             GnPlan p, int B, int act, Drop drop, float2* __restrict__ per_group,
+                                                             float2* __restrict__ per_channel) {
+  constexpr int A = ONE ? 1 : V, E = V / A;
+  __shared__ float2 red[kBlock * V];
+  const Where w = where(p, blockIdx.x);
+  const Rows r(p, w);
+  if (r.mine) {
+    const Stream<DT, V> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r);
+    Raw<DT, V> xr[kU], gr[kU];
+    xs.batch(r, 0, xr);
+    gs.batch(r, 0, gr);
+    const int c = w.c0 + r.vx * V;
+    float mu[A], is[A], ga[V], be[V], s1[V], s2[V];
+#pragma unroll
+    for (int a = 0; a < A; ++a) {
+      const long long g = (long long)w.b * p.G + (c + a * E) / p.cpg;
+      mu[a] = mean[g]; is[a] = rstd[g];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) { ga[k] = gamma[c + k]; be[k] = beta[c + k]; s1[k] = 0.0f; s2[k] = 0.0f; }
+    DropKey key{};
+    unsigned keep = 0;
+    if (DROP) {
+      key = drop_key(drop);
+      if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
+    }
+    const unsigned long long place = (unsigned long long)(w.r0 + r.ry) * p.C + c;
+    for (int t = 0;;) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (t + u >= r.steps) break;
+        if (!r.valid(t + u)) break;
+        float f[V], g[V], z[V];
+        unpack<DT, V>(xr[u], f);
+        unpack<DT, V>(gr[u], g);
+        if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, r, t + u, g);
+        if (DROP) {
+          if (!drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, place + (unsigned long long)(t + u) * p.row_lanes * p.C);
+          drop_apply<V>(g, keep, drop.scale);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
+        act_bwd<V>(g, z, act);
+#pragma unroll
+        for (int k = 0; k < V; ++k) { s1[k] += g[k]; s2[k] = __builtin_fmaf(g[k], f[k], s2[k]); }
+      }
+      t += kU;
+      if (t >= r.steps) break;
+      xs.batch(r, t, xr);
+      gs.batch(r, t, gr);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) red[r.ry * p.cs + r.vx * V + k] = make_float2(s1[k], s2[k]);
+  }
+  __syncthreads();
+  // over the row lanes: S threads per channel take every S-th row lane each, then one adds the S.  In order: the same bits every time.
+  const int S = max(1, kBlock / w.cc);
+  const int cl = threadIdx.x % (unsigned)w.cc, seg = threadIdx.x / (unsigned)w.cc;
+  for (int c = cl; seg < S && c < w.cc; c += kBlock) {  // (cc > kBlock: S = 1 and a thread has several channels)
+    float a = 0.0f, b = 0.0f;
+    for (int l = seg; l < p.row_lanes; l += S) { const float2 v = red[l * p.cs + c]; a += v.x; b += v.y; }
+    if (seg < p.row_lanes) red[seg * p.cs + c] = make_float2(a, b);  // (only this thread reads or writes that place)
+  }
+  __syncthreads();
+  const int left = min(S, p.row_lanes);
+  for (int c = threadIdx.x; c < w.cc; c += kBlock) {
+    float2 v = red[c];
+    for (int l = 1; l < left; ++l) { const float2 o = red[l * p.cs + c]; v.x += o.x; v.y += o.y; }
+    red[c] = v;
+    per_channel[((long long)(w.c0 + c) * B + w.b) * p.chunks + w.chunk] = v;
+  }
+  __syncthreads();
+  const Team t = team_of(w.ng);
+  const int cg = p.parts == 1 ? p.cpg : w.cc;
+  for (int j = t.id; j < w.ng; j += t.count) {
+    float a = 0.0f, b = 0.0f;
+    for (int e = t.lane; e < cg; e += t.T) {
+      const float2 v = red[j * cg + e];
+      const float ga = gamma[w.c0 + j * cg + e];
+      a = __builtin_fmaf(ga, v.x, a);
+      b = __builtin_fmaf(ga, v.y, b);
+    }
+    a = team_sum(a, t.T);
+    b = team_sum(b, t.T);
+    if (t.lane == 0) per_group[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(a, b);
+  }
+}
+
+// ---- backward, second launch: the first param_blocks workgroups sum the channel partials over items and chunks (a wave per
+// channel), the others write gx
+template <int DT, int V, bool ONE, bool DROP, bool FAR>
+__global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+                                                              const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                              GnPlan p, int B, int act, Drop drop,
+                                                              const float2* __restrict__ per_group,
+                                                              const float2* __restrict__ per_channel, unsigned param_blocks,
+                                                              void* __restrict__ gx, float* __restrict__ ggamma,
+                                                              float* __restrict__ gbeta) {
+  constexpr int A = ONE ? 1 : V, E = V / A;
+  __shared__ float2 stat[kBlock * A];
+  if (blockIdx.x < param_blocks) {
+    const int c = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (c >= p.C) return;
+    const long long n = (long long)B * p.chunks;
+    const float2* src = per_channel + c * n;
+    double a = 0.0, b = 0.0;
+    for (long long k = lane; k < n; k += 64) { const float2 v = src[k]; a += v.x; b += v.y; }
+    a = team_sum(a, 64);
+    b = team_sum(b, 64);
+    if (lane == 0) { gbeta[c] = (float)a; ggamma[c] = (float)b; }
+    return;
+  }
+  const Where w = where(p, blockIdx.x - param_blocks);
+  const Rows r(p, w);
+  const Stream<DT, V, FAR> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r), os(gx, p.C, p, w, r);
+  Raw<DT, V> xr[kU], gr[kU];
+  const int c = w.c0 + r.vx * V;
+  float mu[A], is[A], ga[V], be[V], c1[A], c2[A];
+  if (r.mine) {
+    xs.batch(r, 0, xr);
+    gs.batch(r, 0, gr);
+#pragma unroll
+    for (int a = 0; a < A; ++a) {
+      const long long g = (long long)w.b * p.G + (c + a * E) / p.cpg;
+      mu[a] = mean[g]; is[a] = rstd[g];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) { ga[k] = gamma[c + k]; be[k] = beta[c + k]; }
+  }
+  {
+    const Team t = team_of(w.ng);
+    const double inv = 1.0 / ((double)p.N * p.cpg);
+    for (int j = t.id; j < w.ng; j += t.count) {
+      const float2* src = per_group + ((long long)w.b * p.G + w.g0 + j) * p.P;
+      double a = 0.0, b = 0.0;
+      for (int q = t.lane; q < p.P; q += t.T) { const float2 v = src[q]; a += v.x; b += v.y; }
+      a = team_sum(a, t.T);
+      b = team_sum(b, t.T);
+      if (t.lane == 0) stat[j] = make_float2((float)(a * inv), (float)(b * inv));
+    }
+    __syncthreads();
+  }
+  if (!r.mine) return;
+#pragma unroll
+  for (int a = 0; a < A; ++a) {
+    const float2 st = stat[(c + a * E) / p.cpg - w.g0];
+    c1[a] = st.x;
+    c2[a] = st.y;
+  }
+  DropKey key{};
+  unsigned keep = 0;
+  if (DROP) {
+    key = drop_key(drop);
+    if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
+  }
+  const unsigned long long place = (unsigned long long)(w.r0 + r.ry) * p.C + c;
+  for (int t = 0;;) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (t + u >= r.steps) break;
+      float f[V], g[V], z[V];
+      unpack<DT, V>(xr[u], f);
+      unpack<DT, V>(gr[u], g);
+      if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, r, t + u, g);
+      if (DROP) {
+        if (!drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, place + (unsigned long long)(t + u) * p.row_lanes * p.C);
+        drop_apply<V>(g, keep, drop.scale);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
+      act_bwd<V>(g, z, act);
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        g[k] = is[k / E] * __builtin_fmaf(-f[k], c2[k / E], __builtin_fmaf(ga[k], g[k], -c1[k / E]));
+      if (r.valid(t + u)) store_row(os, t + u, g);
+    }
+    t += kU;
+    if (t >= r.steps) break;
+    xs.batch(r, t, xr);
+    gs.batch(r, t, gr);
+  }
+}
+
+}  // namespace
+}  // namespace sfm
+
+using namespace sfm;
+
+extern "C" int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, const void* const* gy, const long long* ld_gy,
+                                      int n_gy, const float* gamma, const float* beta, const float* save_mean,
+                                      const float* save_rstd, long long B, long long N, int C, int G, int act, const void* rng,
+                                      unsigned long long seed, unsigned step, unsigned layer, unsigned item0, int threshold,
+                                      int per_channel, void* gx, float* ggamma, float* gbeta, float* ws, void* stream_) {
+  GnPlan p;
+  Drop d;
+  unsigned grid;
+  const int es = dtype == kF32 ? 4 : 2;
+  if (!gy || !ld_gy || n_gy < 1 || n_gy > 3) return SFM_ERR_ARG;
+  long long ld = ld_x;
+  for (int k = 0; k < n_gy; ++k) ld = std::max(ld, ld_gy[k]);
+  const int rc = gn_setup(B, N, C, G, dtype, ld, p, grid);
+  if (rc) return rc;
+  if (!rows_ok(x, ld_x, C, es) || !gamma || !beta || !save_mean || !save_rstd ||
+      (!gx && !ggamma) || (gx && !rows_ok(gx, C, C, es)) || (!ggamma != !gbeta) || !ws || ((uintptr_t)ws & 7) || act < kActNone ||
+      act > kActSilu || !drop_args(rng, seed, step, layer, item0, threshold, per_channel, d))
+    return SFM_ERR_ARG;
+  if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > 0xffffffffll - item0)) return SFM_ERR_TOO_LARGE;
+  GySrc src{};
+  src.n = n_gy;
+  for (int k = 0; k < n_gy; ++k) {
+    if (!rows_ok(gy[k], ld_gy[k], C, es)) return SFM_ERR_ARG;
+    src.p[k] = gy[k];
+    src.ld[k] = ld_gy[k];
+  }
+  hipStream_t stream = (hipStream_t)stream_;
+  float2* per_group = reinterpret_cast<float2*>(ws);
+  float2* per_channel_sums = per_group + B * G * p.P;
+  const unsigned params = ggamma ? (unsigned)((C + kBlock / 64 - 1) / (kBlock / 64)) : 0u;
+  const unsigned second = params + (gx ? grid : 0u);
+  by_type(dtype, p, [&](auto dt, auto v, auto one) {
+    constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
+    constexpr bool ONE = decltype(one)::value;
+    by_use<DT, V>(threshold != 0, far(3 * B * N * C * es), [&](auto drop, auto away) {
+      constexpr bool DROP = decltype(drop)::value;
+      hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, ONE, DROP>), dim3(grid), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta, save_mean,
+                         save_rstd, p, (int)B, act, d, per_group, per_channel_sums);
+      hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, ONE, DROP, decltype(away)::value>), dim3(second), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta,
+                         save_mean, save_rstd, p, (int)B, act, d, per_group, per_channel_sums, params, gx, ggamma, gbeta);
+    });
+  });
+  return sfm_last_error();
+}

@@ -1,0 +1,229 @@
+// Group norm with an activation: the forward (group_norm.h has the mathematics and the plan).
+#include "group_norm.h"
+
+namespace sfm {
+namespace {
+
+// ---- forward, first launch: part [B][G][P] (mean, M2).  ONE: the V channels of a vector are of one group (V divides cpg), and a
+// thread has one pair for them; else one pair per channel.
+template <int DT, int V, bool ONE>
+__global__ __launch_bounds__(kBlock) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
+                                                          float2* __restrict__ part) {
+  constexpr int A = ONE ? 1 : V, E = V / A;  // accumulators, and elements of one in a row
+  __shared__ float2 red[kBlock * A];         // [row lane][vector or channel of the slab]
+  const Where w = where(p, blockIdx.x);
+  const Rows r(p, w);
+  if (r.mine) {
+    const Stream<DT, V> xs(x, ldx, p, w, r);
+    float n = 0.0f, mean[A], m2[A];
+#pragma unroll
+    for (int a = 0; a < A; ++a) { mean[a] = 0.0f; m2[a] = 0.0f; }
+    Raw<DT, V> raw[kU];
+    int t = 0;
+    for (; t + kU <= r.full; t += kU) {
+      xs.batch(r, t, raw);
+      float s[A], q[A];
+#pragma unroll
+      for (int a = 0; a < A; ++a) { s[a] = 0.0f; q[a] = 0.0f; }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        float f[V];
+        unpack<DT, V>(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[k / E] += f[k];
+      }
+#pragma unroll
+      for (int a = 0; a < A; ++a) s[a] *= 1.0f / (kU * E);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        float f[V];
+        unpack<DT, V>(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) { const float d = f[k] - s[k / E]; q[k / E] = __builtin_fmaf(d, d, q[k / E]); }
+      }
+      const float nn = n + kU * E, share = (kU * E) / nn, cross = n * share;
+#pragma unroll
+      for (int a = 0; a < A; ++a) {
+        const float delta = s[a] - mean[a];
+        mean[a] = __builtin_fmaf(delta, share, mean[a]);
+        m2[a] += __builtin_fmaf(delta * delta, cross, q[a]);
+      }
+      n = nn;
+    }
+    for (; t < r.steps; ++t) {  // fewer than kU steps, and the last one where it is not full
+      if (!r.valid(t)) break;
+      float f[V], s[A], q[A];
+      unpack<DT, V>(xs.load(r, t), f);
+#pragma unroll
+      for (int a = 0; a < A; ++a) { s[a] = 0.0f; q[a] = 0.0f; }
+#pragma unroll
+      for (int k = 0; k < V; ++k) s[k / E] += f[k];
+#pragma unroll
+      for (int a = 0; a < A; ++a) s[a] *= 1.0f / E;
+#pragma unroll
+      for (int k = 0; k < V; ++k) { const float d = f[k] - s[k / E]; q[k / E] = __builtin_fmaf(d, d, q[k / E]); }
+      const float nn = n + E, share = E / nn, cross = n * share;
+#pragma unroll
+      for (int a = 0; a < A; ++a) {
+        const float delta = s[a] - mean[a];
+        mean[a] = __builtin_fmaf(delta, share, mean[a]);
+        m2[a] += __builtin_fmaf(delta * delta, cross, q[a]);
+      }
+      n = nn;
+    }
+#pragma unroll
+    for (int a = 0; a < A; ++a) red[(r.ry * p.lanes + r.vx) * A + a] = make_float2(mean[a], m2[a]);
+  }
+  __syncthreads();
+  // over the row lanes and the vectors of a group.  Means are taken against one of them, so a common part costs no digits.
+  const Team tm = team_of(w.ng);
+  const int per_row = (p.parts == 1 ? p.cpg : w.cc) / E;           // pairs of a group in a row lane
+  const int busy = r.steps > 1 ? p.row_lanes : r.last;             // row lanes that have seen a row
+  const float inv = 1.0f / ((float)w.rows * per_row);
+  for (int j = tm.id; j < w.ng; j += tm.count) {
+    const float ref = red[j * per_row].x;
+    float s = 0.0f;
+    for (int e = tm.lane; e < busy * per_row; e += tm.T) {
+      const int l = e / per_row, c = e - l * per_row;
+      s = __builtin_fmaf((float)(r.steps - 1 + (l < r.last)), red[l * p.lanes * A + j * per_row + c].x - ref, s);
+    }
+    const float off = team_sum(s, tm.T) * inv;
+    float q = 0.0f;
+    for (int e = tm.lane; e < busy * per_row; e += tm.T) {
+      const int l = e / per_row, c = e - l * per_row;
+      const float2 v = red[l * p.lanes * A + j * per_row + c];
+      const float d = (v.x - ref) - off;
+      q += __builtin_fmaf((float)(E * (r.steps - 1 + (l < r.last))) * d, d, v.y);
+    }
+    q = team_sum(q, tm.T);
+    if (tm.lane == 0) part[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(ref + off, q);
+  }
+}
+
+// joins the partials of a workgroup's groups: stat[j] = (mean, r) in LDS.  All threads call it; it ends with a barrier.
+__device__ __forceinline__ void join_stats(const float2* __restrict__ part, const GnPlan& p, const Where& w, float eps,
+                                           float2* __restrict__ stat) {
+  const Team t = team_of(w.ng);
+  const double inv = 1.0 / ((double)p.N * p.cpg);
+  for (int j = t.id; j < w.ng; j += t.count) {
+    const float2* src = part + ((long long)w.b * p.G + w.g0 + j) * p.P;
+    const float ref = src[0].x;
+    double s = 0.0;
+    for (int q = t.lane; q < p.P; q += t.T) s += part_count(p, q) * (src[q].x - ref);
+    const double off = team_sum(s, t.T) * inv;
+    double q2 = 0.0;
+    for (int q = t.lane; q < p.P; q += t.T) {
+      const float2 v = src[q];
+      const double d = (v.x - ref) - off;
+      q2 += v.y + part_count(p, q) * d * d;
+    }
+    q2 = team_sum(q2, t.T);
+    if (t.lane == 0) stat[j] = make_float2((float)(ref + off), (float)(1.0 / sqrt(q2 * inv + (double)eps)));
+  }
+  __syncthreads();
+}
+
+// ---- forward, second launch.  The first batch is on its way while the partials are joined.
+template <int DT, int V, bool ONE, bool DROP, bool FAR>
+__global__ __launch_bounds__(kBlock) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
+                                                          const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                          const float2* __restrict__ part, GnPlan p, float eps, int act, Drop drop,
+                                                          void* __restrict__ y, long long ldy, float* __restrict__ save_mean,
+                                                          float* __restrict__ save_r) {
+  constexpr int A = ONE ? 1 : V, E = V / A;
+  __shared__ float2 stat[kBlock * A];
+  const Where w = where(p, blockIdx.x);
+  const Rows r(p, w);
+  const Stream<DT, V, FAR> xs(x, ldx, p, w, r), ys(y, ldy, p, w, r);
+  Raw<DT, V> raw[kU];
+  float sc[V], sh[V];
+  const int c = w.c0 + r.vx * V;
+  if (r.mine) {
+    xs.batch(r, 0, raw);
+#pragma unroll
+    for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k]; sh[k] = beta[c + k]; }
+  }
+  join_stats(part, p, w, eps, stat);
+  if (save_mean && w.chunk == 0 && w.part == 0)
+    for (int j = threadIdx.x; j < w.ng; j += kBlock) {
+      save_mean[(long long)w.b * p.G + w.g0 + j] = stat[j].x;
+      save_r[(long long)w.b * p.G + w.g0 + j] = stat[j].y;
+    }
+  if (!r.mine) return;
+  float mu[A];
+#pragma unroll
+  for (int a = 0; a < A; ++a) {
+    const float2 st = stat[(c + a * E) / p.cpg - w.g0];
+    mu[a] = st.x;
+#pragma unroll
+    for (int k = a * E; k < (a + 1) * E; ++k) sc[k] *= st.y;
+  }
+  DropKey key{};
+  unsigned keep = 0;
+  if (DROP) {
+    key = drop_key(drop);
+    if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
+  }
+  const unsigned long long place = (unsigned long long)(w.r0 + r.ry) * p.C + c;
+  for (int t = 0;;) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (t + u >= r.steps) break;
+      float f[V];
+      unpack<DT, V>(raw[u], f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
+      act_fwd<V>(f, act);
+      if (DROP) {
+        if (!drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, place + (unsigned long long)(t + u) * p.row_lanes * p.C);
+        drop_apply<V>(f, keep, drop.scale);
+      }
+      if (r.valid(t + u)) store_row(ys, t + u, f);
+    }
+    t += kU;
+    if (t >= r.steps) break;
+    xs.batch(r, t, raw);
+  }
+}
+
+}  // namespace
+}  // namespace sfm
+
+using namespace sfm;
+
+extern "C" long long sfm_group_norm_workspace_floats(long long B, long long N, int C, int G, int dtype, int backward) {
+  GnPlan p;
+  unsigned grid;
+  const int rc = gn_setup(B, N, C, G, dtype, C, p, grid);
+  if (rc) return rc;
+  return 2 * (B * G * p.P + (backward ? B * C * p.chunks : 0));
+}
+
+extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, const float* gamma, const float* beta, long long B,
+                                      long long N, int C, int G, float eps, int act, const void* rng, unsigned long long seed,
+                                      unsigned step, unsigned layer, unsigned item0, int threshold, int per_channel, void* y,
+                                      long long ld_y, float* save_mean, float* save_rstd, float* ws, void* stream_) {
+  GnPlan p;
+  Drop d;
+  unsigned grid;
+  const int es = dtype == kF32 ? 4 : 2;
+  const int rc = gn_setup(B, N, C, G, dtype, std::max(ld_x, ld_y), p, grid);
+  if (rc) return rc;
+  if (!rows_ok(x, ld_x, C, es) || !rows_ok(y, ld_y, C, es) || !gamma || !beta || !ws || ((uintptr_t)ws & 7) || !(eps > 0.0f) ||
+      act < kActNone || act > kActSilu || (!save_mean != !save_rstd) ||
+      !drop_args(rng, seed, step, layer, item0, threshold, per_channel, d))
+    return SFM_ERR_ARG;
+  if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > 0xffffffffll - item0)) return SFM_ERR_TOO_LARGE;
+  hipStream_t stream = (hipStream_t)stream_;
+  float2* part = reinterpret_cast<float2*>(ws);
+  by_type(dtype, p, [&](auto dt, auto v, auto one) {
+    constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
+    constexpr bool ONE = decltype(one)::value;
+    hipLaunchKernelGGL((gn_stats_kernel<DT, V, ONE>), dim3(grid), dim3(kBlock), 0, stream, x, ld_x, p, part);
+    by_use<DT, V>(threshold != 0, far(2 * B * N * C * es), [&](auto drop, auto away) {
+      hipLaunchKernelGGL((gn_apply_kernel<DT, V, ONE, decltype(drop)::value, decltype(away)::value>), dim3(grid), dim3(kBlock), 0, stream,
+                         x, ld_x, gamma, beta, part, p, eps, act, d, y, ld_y, save_mean, save_rstd);
+    });
+  });
+  return sfm_last_error();
+}
