@@ -23,10 +23,13 @@ namespace {
 
 
 constexpr int kTargetBlocks = 1024;  // four workgroups of four waves per CU: all of a launch is resident (2048 was two rounds of most kernels)
-constexpr int kMaxChunks = 512;
-constexpr int kU = 4;                  // rows a thread has in flight
+constexpr int kMaxChunks = 1024;
+constexpr int kU = 4;  // rows a thread has in flight
 
-// How an item is cut: channels into slabs (whole groups, or an even part of one wide group), rows into chunks.
+// How an item is cut: channels into slabs (whole groups, or an even part of one wide group), rows into tiles of kU * row_lanes
+// rows, and the tiles in turn to the chunks (tile t to chunk t % chunks), one workgroup each.  In turn and not in runs: the
+// workgroups then move through memory side by side.  Passes over tensors of 512 MB, nontemporal: read + write 175 us in turn, 190 in
+// runs; two reads + write 263 and 283.
 struct GnPlan {
   long long N;
   int C, G, cpg;
@@ -38,8 +41,13 @@ struct GnPlan {
   int lanes;             // cs / V
   int row_lanes;         // kBlock / lanes: rows a workgroup takes at once
   int chunks;
-  int rows_per_chunk;
   int P;                 // partials of a group: chunks * parts
+  // rows into tiles and chunks (gn_tiles)
+  int tile_rows;
+  long long tiles;
+  long long own;         // tiles of a chunk; the first `extra` chunks have one more
+  int extra;
+  int owner, left;       // the chunk of the last tile, and the rows of that tile
 };
 
 static inline int gcd_int(int a, int b) {
@@ -47,8 +55,21 @@ static inline int gcd_int(int a, int b) {
   return a;
 }
 
+// (also after the number of chunks is known: a row stride may ask for fewer row lanes, which makes more tiles of the same chunks)
+static void gn_tiles(GnPlan& p, int row_lanes) {
+  p.row_lanes = row_lanes;
+  p.tile_rows = kU * row_lanes;
+  p.tiles = (p.N + p.tile_rows - 1) / p.tile_rows;
+  if (p.chunks < 1) p.chunks = 1;
+  p.own = p.tiles / p.chunks;
+  p.extra = (int)(p.tiles % p.chunks);
+  p.owner = (int)((p.tiles - 1) % p.chunks);
+  p.left = (int)(p.N - (p.tiles - 1) * p.tile_rows);
+}
+
 // (the arguments have been checked; false: an item is too large)
 static bool gn_plan(long long B, long long N, int C, int G, int es, GnPlan& p) {
+  p = GnPlan{};
   p.N = N; p.C = C; p.G = G; p.cpg = C / G;
   p.V = 16 / es;
   while (C % p.V) p.V /= 2;
@@ -78,19 +99,13 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, GnPlan& p) {
     p.slabs = G * p.parts;
   }
   p.lanes = p.cs / p.V;
-  p.row_lanes = kBlock / p.lanes;
-  const long long per = (long long)B * p.slabs, step = (long long)kU * p.row_lanes;
-  long long chunks = (kTargetBlocks + per - 1) / per;
-  const long long most = (N + step - 1) / step;  // a full batch per thread at least
-  if (chunks > most) chunks = most;
-  if (chunks > kMaxChunks) chunks = kMaxChunks;
-  if (chunks < 1) chunks = 1;
-  long long rows = (N + chunks - 1) / chunks;
-  if (rows > step) rows = (rows + step - 1) / step * step;  // whole batches in all chunks but the last
-  if (rows > 0x7fffffffll) return false;
-  p.rows_per_chunk = (int)rows;
-  p.chunks = (int)((N + rows - 1) / rows);
+  gn_tiles(p, kBlock / p.lanes);
+  const long long per = (long long)B * p.slabs;
+  long long chunks = std::min({(kTargetBlocks + per - 1) / per, p.tiles, (long long)kMaxChunks});
+  const long long each = (p.tiles + chunks - 1) / chunks;  // as even as whole tiles allow
+  p.chunks = (int)((p.tiles + each - 1) / each);
   p.P = p.chunks * p.parts;
+  gn_tiles(p, p.row_lanes);
   return true;
 }
 
@@ -98,8 +113,6 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, GnPlan& p) {
 struct Where {
   int b, slab, chunk, part;
   int c0, cc, g0, ng;  // first channel and channels of the slab, first group and groups of it
-  long long r0;        // first row, in the item
-  int rows;
 };
 __device__ __forceinline__ Where where(const GnPlan& p, unsigned bid) {
   Where w;
@@ -120,62 +133,65 @@ __device__ __forceinline__ Where where(const GnPlan& p, unsigned bid) {
     w.c0 = w.g0 * p.cpg + w.part * p.cs;
     w.cc = min(p.cs, p.cpg - w.part * p.cs);
   }
-  w.r0 = (long long)w.chunk * p.rows_per_chunk;
-  w.rows = (int)min((long long)p.rows_per_chunk, p.N - w.r0);
   return w;
 }
 
-// The rows of a thread: vector vx of the slab in rows ry, ry + row_lanes, ... of the chunk, one per step, in batches of kU steps.  The
-// address of a load is a uniform pointer that moves with the step and a 32-bit offset of the thread (gn_setup keeps row_lanes rows
-// under 2^31 bytes).
-struct Rows {
+// A tile's rows go to the row lanes in kU steps: step u, row lane ry: row u * row_lanes + ry of the tile.  Everything here but
+// the thread's own place is uniform: the address of a load is a uniform pointer and a 32-bit offset of the thread (gn_setup
+// keeps the rows of a step within 31 bits of bytes).
+struct Lane {
   int vx, ry;
-  bool mine;     // this thread has a vector at all
-  int steps;     // of the chunk
-  int last;      // rows of its last step (1 .. row_lanes)
-  int full;      // steps in which every row lane has a row
-  __device__ __forceinline__ Rows(const GnPlan& p, const Where& w) {
+  bool mine;  // this thread has a vector at all
+  __device__ __forceinline__ Lane(const GnPlan& p, const Where& w) {
     vx = threadIdx.x % (unsigned)p.lanes;
     ry = threadIdx.x / (unsigned)p.lanes;
     mine = ry < p.row_lanes && vx * p.V < w.cc;
-    steps = (w.rows + p.row_lanes - 1) / p.row_lanes;
-    last = w.rows - (steps - 1) * p.row_lanes;
-    full = last == p.row_lanes ? steps : steps - 1;
   }
-  __device__ __forceinline__ bool valid(int t) const { return t < steps - 1 || (t == steps - 1 && ry < last); }
+};
+struct Tile {
+  long long index;
+  int steps;  // steps in which row lane 0 has a row
+  int last;   // rows of the last of them (1 .. row_lanes)
+  bool full;
+  __device__ __forceinline__ Tile(const GnPlan& p, long long i) : index(i) {
+    full = i < p.tiles - 1 || p.left == p.tile_rows;
+    steps = full ? kU : (p.left + p.row_lanes - 1) / p.row_lanes;
+    last = full ? p.row_lanes : p.left - (steps - 1) * p.row_lanes;
+  }
+  __device__ __forceinline__ bool valid(int u, int ry) const { return full || u < steps - 1 || (u == steps - 1 && ry < last); }
 };
 
-// NT: nontemporal, for tensors that no cache holds until they are read again (far(), below)
-template <int DT, int V, bool NT = false> struct Stream {
+template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, for tensors that no cache holds until they are read again (far(), below)
   static constexpr int kES = ElemBytes<DT>::value;
   const char* base;
-  long long step;
-  unsigned off, back;  // back: in the last step a row lane without a row reads row lane 0's
-  __device__ __forceinline__ Stream(const void* p, long long ld, const GnPlan& pl, const Where& w, const Rows& r) {
-    base = static_cast<const char*>(p) + (((long long)w.b * pl.N + w.r0) * ld + w.c0) * kES;
+  long long step;      // bytes of the rows of a step
+  unsigned off, lead;  // of this thread; lead: its row lane's share of it
+  __device__ __forceinline__ Stream(const void* p, long long ld, const GnPlan& pl, const Where& w, const Lane& l) {
+    base = static_cast<const char*>(p) + ((long long)w.b * pl.N * ld + w.c0) * kES;
     step = (long long)pl.row_lanes * ld * kES;
-    off = (unsigned)((r.ry * ld + r.vx * V) * kES);
-    back = r.ry < r.last ? 0u : (unsigned)(r.ry * ld * kES);
+    lead = (unsigned)(l.ry * ld * kES);
+    off = lead + (unsigned)(l.vx * V * kES);
   }
-  __device__ __forceinline__ Raw<DT, V> load(const Rows& r, int t) const {  // t < r.steps, uniform
-    return load_raw<DT, V, NT>(base + t * step, off - (t < r.steps - 1 ? 0u : back));
+  __device__ __forceinline__ const char* at(const Tile& t, int u) const { return base + (t.index * kU + u) * step; }
+  // one row of the tile, u < steps; in its last step a row lane without a row reads row lane 0's
+  __device__ __forceinline__ Raw<DT, V> row(const Tile& t, int u, int ry) const {
+    return load_raw<DT, V, NT>(at(t, u), off - (t.valid(u, ry) ? 0u : lead));
   }
-  __device__ __forceinline__ void batch(const Rows& r, int t0, Raw<DT, V> (&raw)[kU]) const {
-    if (t0 + kU <= r.full) {
-      const char* at = base + t0 * step;
+  __device__ __forceinline__ void load(const Tile& t, int ry, Raw<DT, V> (&raw)[kU]) const {
+    if (t.full) {
+      const char* a = at(t, 0);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) { raw[u] = load_raw<DT, V, NT>(at, off); at += step; }
+      for (int u = 0; u < kU; ++u) { raw[u] = load_raw<DT, V, NT>(a, off); a += step; }
     } else {
 #pragma unroll
       for (int u = 0; u < kU; ++u)
-        if (t0 + u < r.steps) raw[u] = load(r, t0 + u);
+        if (u < t.steps) raw[u] = row(t, u, ry);
     }
   }
+  __device__ __forceinline__ void store(const Tile& t, int u, const float (&f)[V]) const {
+    store_vec<DT, V, NT>(const_cast<char*>(at(t, u)), off, f);
+  }
 };
-template <int DT, int V, bool NT>
-__device__ __forceinline__ void store_row(const Stream<DT, V, NT>& s, int t, const float (&f)[V]) {
-  store_vec<DT, V, NT>(const_cast<char*>(s.base) + t * s.step, s.off, f);
-}
 
 // Teams: the workgroup's threads, cut into teams of T lanes of one wave (T a power of two), one group each at a time.
 struct Team { int T, id, lane, count; };
@@ -192,8 +208,8 @@ template <typename F> __device__ __forceinline__ F team_sum(F v, int T) {
 // values that partial q of a group covers
 __device__ __forceinline__ double part_count(const GnPlan& p, int q) {
   const int chunk = p.parts == 1 ? q : q / p.parts, part = q - chunk * p.parts;
-  const int rows = chunk == p.chunks - 1 ? (int)(p.N - (long long)chunk * p.rows_per_chunk) : p.rows_per_chunk;
-  return (double)rows * (p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
+  const double rows = (double)((p.own + (chunk < p.extra)) * p.tile_rows - (chunk == p.owner ? p.tile_rows - p.left : 0));
+  return rows * (p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
 }
 
 // dispatch on the type, the vector width and whether a vector lies in one group: fn(DT, V, ONE) as integral constants
@@ -242,7 +258,7 @@ static int gn_setup(long long B, long long N, int C, int G, int dtype, long long
   // lie within 31 bits of bytes of each other
   if (B > 0x7fffffffll || (__int128)B * N > ((__int128)1 << 40) || ld > 0x7fffffffll / es || !gn_plan(B, N, C, G, es, p))
     return SFM_ERR_TOO_LARGE;
-  p.row_lanes = (int)std::min<long long>(p.row_lanes, 0x7fffffffll / (ld * es));
+  gn_tiles(p, (int)std::min<long long>(p.row_lanes, 0x7fffffffll / (ld * es)));
   const __int128 blocks = (__int128)B * p.slabs * p.chunks;
   if (blocks + C > 0x7fffffffll) return SFM_ERR_TOO_LARGE;
   grid = (unsigned)blocks;

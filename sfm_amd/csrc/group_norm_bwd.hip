@@ -12,11 +12,12 @@ struct GySrc {
   int n;
 };
 template <int DT, int V>
-__device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, const Where& w, const Rows& r, int t, float (&g)[V]) {
+__device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, const Where& w, const Lane& l, const Tile& t, int u,
+                                            float (&g)[V]) {
   for (int k = 1; k < s.n; ++k) {  // uniform
-    const Stream<DT, V> more(s.p[k], s.ld[k], p, w, r);
+    const Stream<DT, V> more(s.p[k], s.ld[k], p, w, l);
     float f[V];
-    unpack<DT, V>(more.load(r, t), f);
+    unpack<DT, V>(more.row(t, u, l.ry), f);
 #pragma unroll
     for (int e = 0; e < V; ++e) g[e] += f[e];
   }
@@ -24,7 +25,7 @@ __device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, con
 
 // ---- backward, first launch: per_group [B][G][P] (sum gamma dz, sum gamma dz xhat), per_channel [C][B][chunks] (sum dz, sum dz xhat)
 template <int DT, int V, bool ONE, bool DROP>
-__global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+__global__ __launch_bounds__(kBlock, 4) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                              const float* __restrict__ gamma, const float* __restrict__ beta,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
                                                              GnPlan p, int B, int act, Drop drop, float2* __restrict__ per_group,
@@ -32,13 +33,14 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restr
   constexpr int A = ONE ? 1 : V, E = V / A;
   __shared__ float2 red[kBlock * V];
   const Where w = where(p, blockIdx.x);
-  const Rows r(p, w);
-  if (r.mine) {
-    const Stream<DT, V> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r);
+  const Lane l(p, w);
+  if (l.mine) {
+    const Stream<DT, V> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l);
+    Tile t(p, w.chunk);
     Raw<DT, V> xr[kU], gr[kU];
-    xs.batch(r, 0, xr);
-    gs.batch(r, 0, gr);
-    const int c = w.c0 + r.vx * V;
+    xs.load(t, l.ry, xr);
+    gs.load(t, l.ry, gr);
+    const int c = w.c0 + l.vx * V;
     float mu[A], is[A], ga[V], be[V], s1[V], s2[V];
 #pragma unroll
     for (int a = 0; a < A; ++a) {
@@ -53,18 +55,18 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restr
       key = drop_key(drop);
       if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
     }
-    const unsigned long long place = (unsigned long long)(w.r0 + r.ry) * p.C + c;
-    for (int t = 0;;) {
+    const unsigned long long place = (unsigned long long)l.ry * p.C + c;
+    for (;;) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        if (t + u >= r.steps) break;
-        if (!r.valid(t + u)) break;
+        if (u >= t.steps || !t.valid(u, l.ry)) break;
         float f[V], g[V], z[V];
         unpack<DT, V>(xr[u], f);
         unpack<DT, V>(gr[u], g);
-        if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, r, t + u, g);
+        if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, l, t, u, g);
         if (DROP) {
-          if (!drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, place + (unsigned long long)(t + u) * p.row_lanes * p.C);
+          if (!drop.per_channel)
+            keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
           drop_apply<V>(g, keep, drop.scale);
         }
 #pragma unroll
@@ -73,13 +75,13 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restr
 #pragma unroll
         for (int k = 0; k < V; ++k) { s1[k] += g[k]; s2[k] = __builtin_fmaf(g[k], f[k], s2[k]); }
       }
-      t += kU;
-      if (t >= r.steps) break;
-      xs.batch(r, t, xr);
-      gs.batch(r, t, gr);
+      if (t.index + p.chunks >= p.tiles) break;
+      t = Tile(p, t.index + p.chunks);
+      xs.load(t, l.ry, xr);
+      gs.load(t, l.ry, gr);
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) red[r.ry * p.cs + r.vx * V + k] = make_float2(s1[k], s2[k]);
+    for (int k = 0; k < V; ++k) red[l.ry * p.cs + l.vx * V + k] = make_float2(s1[k], s2[k]);
   }
   __syncthreads();
   // over the row lanes: S threads per channel take every S-th row lane each, then one adds the S.  In order: the same bits every time.
@@ -87,38 +89,38 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const void* __restr
   const int cl = threadIdx.x % (unsigned)w.cc, seg = threadIdx.x / (unsigned)w.cc;
   for (int c = cl; seg < S && c < w.cc; c += kBlock) {  // (cc > kBlock: S = 1 and a thread has several channels)
     float a = 0.0f, b = 0.0f;
-    for (int l = seg; l < p.row_lanes; l += S) { const float2 v = red[l * p.cs + c]; a += v.x; b += v.y; }
+    for (int i = seg; i < p.row_lanes; i += S) { const float2 v = red[i * p.cs + c]; a += v.x; b += v.y; }
     if (seg < p.row_lanes) red[seg * p.cs + c] = make_float2(a, b);  // (only this thread reads or writes that place)
   }
   __syncthreads();
   const int left = min(S, p.row_lanes);
   for (int c = threadIdx.x; c < w.cc; c += kBlock) {
     float2 v = red[c];
-    for (int l = 1; l < left; ++l) { const float2 o = red[l * p.cs + c]; v.x += o.x; v.y += o.y; }
+    for (int i = 1; i < left; ++i) { const float2 o = red[i * p.cs + c]; v.x += o.x; v.y += o.y; }
     red[c] = v;
     per_channel[((long long)(w.c0 + c) * B + w.b) * p.chunks + w.chunk] = v;
   }
   __syncthreads();
-  const Team t = team_of(w.ng);
+  const Team tm = team_of(w.ng);
   const int cg = p.parts == 1 ? p.cpg : w.cc;
-  for (int j = t.id; j < w.ng; j += t.count) {
+  for (int j = tm.id; j < w.ng; j += tm.count) {
     float a = 0.0f, b = 0.0f;
-    for (int e = t.lane; e < cg; e += t.T) {
+    for (int e = tm.lane; e < cg; e += tm.T) {
       const float2 v = red[j * cg + e];
       const float ga = gamma[w.c0 + j * cg + e];
       a = __builtin_fmaf(ga, v.x, a);
       b = __builtin_fmaf(ga, v.y, b);
     }
-    a = team_sum(a, t.T);
-    b = team_sum(b, t.T);
-    if (t.lane == 0) per_group[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(a, b);
+    a = team_sum(a, tm.T);
+    b = team_sum(b, tm.T);
+    if (tm.lane == 0) per_group[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(a, b);
   }
 }
 
 // ---- backward, second launch: the first param_blocks workgroups sum the channel partials over items and chunks (a wave per
 // channel), the others write gx
 template <int DT, int V, bool ONE, bool DROP, bool FAR>
-__global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+__global__ __launch_bounds__(kBlock, 4) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
                                                               GnPlan p, int B, int act, Drop drop,
@@ -141,14 +143,15 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __rest
     return;
   }
   const Where w = where(p, blockIdx.x - param_blocks);
-  const Rows r(p, w);
-  const Stream<DT, V, FAR> xs(x, ldx, p, w, r), gs(gy.p[0], gy.ld[0], p, w, r), os(gx, p.C, p, w, r);
+  const Lane l(p, w);
+  const Stream<DT, V, FAR> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l), os(gx, p.C, p, w, l);
+  Tile t(p, w.chunk);
   Raw<DT, V> xr[kU], gr[kU];
-  const int c = w.c0 + r.vx * V;
+  const int c = w.c0 + l.vx * V;
   float mu[A], is[A], ga[V], be[V], c1[A], c2[A];
-  if (r.mine) {
-    xs.batch(r, 0, xr);
-    gs.batch(r, 0, gr);
+  if (l.mine) {
+    xs.load(t, l.ry, xr);
+    gs.load(t, l.ry, gr);
 #pragma unroll
     for (int a = 0; a < A; ++a) {
       const long long g = (long long)w.b * p.G + (c + a * E) / p.cpg;
@@ -158,19 +161,19 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __rest
     for (int k = 0; k < V; ++k) { ga[k] = gamma[c + k]; be[k] = beta[c + k]; }
   }
   {
-    const Team t = team_of(w.ng);
+    const Team tm = team_of(w.ng);
     const double inv = 1.0 / ((double)p.N * p.cpg);
-    for (int j = t.id; j < w.ng; j += t.count) {
+    for (int j = tm.id; j < w.ng; j += tm.count) {
       const float2* src = per_group + ((long long)w.b * p.G + w.g0 + j) * p.P;
       double a = 0.0, b = 0.0;
-      for (int q = t.lane; q < p.P; q += t.T) { const float2 v = src[q]; a += v.x; b += v.y; }
-      a = team_sum(a, t.T);
-      b = team_sum(b, t.T);
-      if (t.lane == 0) stat[j] = make_float2((float)(a * inv), (float)(b * inv));
+      for (int q = tm.lane; q < p.P; q += tm.T) { const float2 v = src[q]; a += v.x; b += v.y; }
+      a = team_sum(a, tm.T);
+      b = team_sum(b, tm.T);
+      if (tm.lane == 0) stat[j] = make_float2((float)(a * inv), (float)(b * inv));
     }
     __syncthreads();
   }
-  if (!r.mine) return;
+  if (!l.mine) return;
 #pragma unroll
   for (int a = 0; a < A; ++a) {
     const float2 st = stat[(c + a * E) / p.cpg - w.g0];
@@ -183,17 +186,18 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __rest
     key = drop_key(drop);
     if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
   }
-  const unsigned long long place = (unsigned long long)(w.r0 + r.ry) * p.C + c;
-  for (int t = 0;;) {
+  const unsigned long long place = (unsigned long long)l.ry * p.C + c;
+  for (;;) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (t + u >= r.steps) break;
+      if (u >= t.steps) break;
       float f[V], g[V], z[V];
       unpack<DT, V>(xr[u], f);
       unpack<DT, V>(gr[u], g);
-      if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, r, t + u, g);
+      if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, l, t, u, g);
       if (DROP) {
-        if (!drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, place + (unsigned long long)(t + u) * p.row_lanes * p.C);
+        if (!drop.per_channel)
+          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
         drop_apply<V>(g, keep, drop.scale);
       }
 #pragma unroll
@@ -202,12 +206,12 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const void* __rest
 #pragma unroll
       for (int k = 0; k < V; ++k)
         g[k] = is[k / E] * __builtin_fmaf(-f[k], c2[k / E], __builtin_fmaf(ga[k], g[k], -c1[k / E]));
-      if (r.valid(t + u)) store_row(os, t + u, g);
+      if (t.valid(u, l.ry)) os.store(t, u, g);
     }
-    t += kU;
-    if (t >= r.steps) break;
-    xs.batch(r, t, xr);
-    gs.batch(r, t, gr);
+    if (t.index + p.chunks >= p.tiles) break;
+    t = Tile(p, t.index + p.chunks);
+    xs.load(t, l.ry, xr);
+    gs.load(t, l.ry, gr);
   }
 }
 

@@ -7,41 +7,40 @@ namespace {
 // ---- forward, first launch: part [B][G][P] (mean, M2).  ONE: the V channels of a vector are of one group (V divides cpg), and a
 // thread has one pair for them; else one pair per channel.
 template <int DT, int V, bool ONE>
-__global__ __launch_bounds__(kBlock) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
+__global__ __launch_bounds__(kBlock, 4) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
                                                           float2* __restrict__ part) {
   constexpr int A = ONE ? 1 : V, E = V / A;  // accumulators, and elements of one in a row
   __shared__ float2 red[kBlock * A];         // [row lane][vector or channel of the slab]
   const Where w = where(p, blockIdx.x);
-  const Rows r(p, w);
-  if (r.mine) {
-    const Stream<DT, V> xs(x, ldx, p, w, r);
+  const Lane l(p, w);
+  if (l.mine) {
+    const Stream<DT, V> xs(x, ldx, p, w, l);
     float n = 0.0f, mean[A], m2[A];
 #pragma unroll
     for (int a = 0; a < A; ++a) { mean[a] = 0.0f; m2[a] = 0.0f; }
-    Raw<DT, V> raw[kU];
-    int t = 0;
-    for (; t + kU <= r.full; t += kU) {
-      xs.batch(r, t, raw);
+    // a batch of R rows: its mean, its squared deviations from that, joined to (n, mean, m2)
+    auto join = [&](auto rows, const Raw<DT, V>* raw) {
+      constexpr int R = decltype(rows)::value;
       float s[A], q[A];
 #pragma unroll
       for (int a = 0; a < A; ++a) { s[a] = 0.0f; q[a] = 0.0f; }
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
+      for (int u = 0; u < R; ++u) {
         float f[V];
         unpack<DT, V>(raw[u], f);
 #pragma unroll
         for (int k = 0; k < V; ++k) s[k / E] += f[k];
       }
 #pragma unroll
-      for (int a = 0; a < A; ++a) s[a] *= 1.0f / (kU * E);
+      for (int a = 0; a < A; ++a) s[a] *= 1.0f / (R * E);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
+      for (int u = 0; u < R; ++u) {
         float f[V];
         unpack<DT, V>(raw[u], f);
 #pragma unroll
         for (int k = 0; k < V; ++k) { const float d = f[k] - s[k / E]; q[k / E] = __builtin_fmaf(d, d, q[k / E]); }
       }
-      const float nn = n + kU * E, share = (kU * E) / nn, cross = n * share;
+      const float nn = n + R * E, share = (R * E) / nn, cross = n * share;
 #pragma unroll
       for (int a = 0; a < A; ++a) {
         const float delta = s[a] - mean[a];
@@ -49,51 +48,45 @@ __global__ __launch_bounds__(kBlock) void gn_stats_kernel(const void* __restrict
         m2[a] += __builtin_fmaf(delta * delta, cross, q[a]);
       }
       n = nn;
-    }
-    for (; t < r.steps; ++t) {  // fewer than kU steps, and the last one where it is not full
-      if (!r.valid(t)) break;
-      float f[V], s[A], q[A];
-      unpack<DT, V>(xs.load(r, t), f);
+    };
+    for (long long i = w.chunk; i < p.tiles; i += p.chunks) {
+      const Tile t(p, i);
+      Raw<DT, V> raw[kU];
+      xs.load(t, l.ry, raw);
+      if (t.full) join(std::integral_constant<int, kU>{}, raw);
+      else {
 #pragma unroll
-      for (int a = 0; a < A; ++a) { s[a] = 0.0f; q[a] = 0.0f; }
-#pragma unroll
-      for (int k = 0; k < V; ++k) s[k / E] += f[k];
-#pragma unroll
-      for (int a = 0; a < A; ++a) s[a] *= 1.0f / E;
-#pragma unroll
-      for (int k = 0; k < V; ++k) { const float d = f[k] - s[k / E]; q[k / E] = __builtin_fmaf(d, d, q[k / E]); }
-      const float nn = n + E, share = E / nn, cross = n * share;
-#pragma unroll
-      for (int a = 0; a < A; ++a) {
-        const float delta = s[a] - mean[a];
-        mean[a] = __builtin_fmaf(delta, share, mean[a]);
-        m2[a] += __builtin_fmaf(delta * delta, cross, q[a]);
+        for (int u = 0; u < kU; ++u)
+          if (u < t.steps && t.valid(u, l.ry)) join(std::integral_constant<int, 1>{}, raw + u);
       }
-      n = nn;
     }
 #pragma unroll
-    for (int a = 0; a < A; ++a) red[(r.ry * p.lanes + r.vx) * A + a] = make_float2(mean[a], m2[a]);
+    for (int a = 0; a < A; ++a) red[(l.ry * p.lanes + l.vx) * A + a] = make_float2(mean[a], m2[a]);
   }
   __syncthreads();
   // over the row lanes and the vectors of a group.  Means are taken against one of them, so a common part costs no digits.
   const Team tm = team_of(w.ng);
   const int per_row = (p.parts == 1 ? p.cpg : w.cc) / E;           // pairs of a group in a row lane
-  const int busy = r.steps > 1 ? p.row_lanes : r.last;             // row lanes that have seen a row
-  const float inv = 1.0f / ((float)w.rows * per_row);
+  const bool partial = w.chunk == p.owner && p.left < p.tile_rows;
+  const long long whole = p.own + (w.chunk < p.extra) - partial;   // whole tiles of this chunk
+  const int tail = partial ? p.left / p.row_lanes : 0, more = partial ? p.left % p.row_lanes : 0;
+  const float rows = (float)(whole * kU + tail);                   // of a row lane; the first `more` lanes have one more
+  const int busy = whole > 0 || tail > 0 ? p.row_lanes : more;     // row lanes that have seen a row
+  const float inv = 1.0f / ((rows * p.row_lanes + more) * per_row);
   for (int j = tm.id; j < w.ng; j += tm.count) {
     const float ref = red[j * per_row].x;
     float s = 0.0f;
     for (int e = tm.lane; e < busy * per_row; e += tm.T) {
-      const int l = e / per_row, c = e - l * per_row;
-      s = __builtin_fmaf((float)(r.steps - 1 + (l < r.last)), red[l * p.lanes * A + j * per_row + c].x - ref, s);
+      const int row = e / per_row, c = e - row * per_row;
+      s = __builtin_fmaf(rows + (row < more), red[row * p.lanes * A + j * per_row + c].x - ref, s);
     }
     const float off = team_sum(s, tm.T) * inv;
     float q = 0.0f;
     for (int e = tm.lane; e < busy * per_row; e += tm.T) {
-      const int l = e / per_row, c = e - l * per_row;
-      const float2 v = red[l * p.lanes * A + j * per_row + c];
+      const int row = e / per_row, c = e - row * per_row;
+      const float2 v = red[row * p.lanes * A + j * per_row + c];
       const float d = (v.x - ref) - off;
-      q += __builtin_fmaf((float)(E * (r.steps - 1 + (l < r.last))) * d, d, v.y);
+      q += __builtin_fmaf(E * (rows + (row < more)) * d, d, v.y);
     }
     q = team_sum(q, tm.T);
     if (tm.lane == 0) part[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(ref + off, q);
@@ -125,7 +118,7 @@ __device__ __forceinline__ void join_stats(const float2* __restrict__ part, cons
 
 // ---- forward, second launch.  The first batch is on its way while the partials are joined.
 template <int DT, int V, bool ONE, bool DROP, bool FAR>
-__global__ __launch_bounds__(kBlock) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
+__global__ __launch_bounds__(kBlock, 4) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
                                                           const float2* __restrict__ part, GnPlan p, float eps, int act, Drop drop,
                                                           void* __restrict__ y, long long ldy, float* __restrict__ save_mean,
@@ -133,13 +126,14 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const void* __restrict
   constexpr int A = ONE ? 1 : V, E = V / A;
   __shared__ float2 stat[kBlock * A];
   const Where w = where(p, blockIdx.x);
-  const Rows r(p, w);
-  const Stream<DT, V, FAR> xs(x, ldx, p, w, r), ys(y, ldy, p, w, r);
+  const Lane l(p, w);
+  const Stream<DT, V, FAR> xs(x, ldx, p, w, l), ys(y, ldy, p, w, l);
+  Tile t(p, w.chunk);
   Raw<DT, V> raw[kU];
   float sc[V], sh[V];
-  const int c = w.c0 + r.vx * V;
-  if (r.mine) {
-    xs.batch(r, 0, raw);
+  const int c = w.c0 + l.vx * V;
+  if (l.mine) {
+    xs.load(t, l.ry, raw);
 #pragma unroll
     for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k]; sh[k] = beta[c + k]; }
   }
@@ -149,7 +143,7 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const void* __restrict
       save_mean[(long long)w.b * p.G + w.g0 + j] = stat[j].x;
       save_r[(long long)w.b * p.G + w.g0 + j] = stat[j].y;
     }
-  if (!r.mine) return;
+  if (!l.mine) return;
   float mu[A];
 #pragma unroll
   for (int a = 0; a < A; ++a) {
@@ -164,25 +158,26 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const void* __restrict
     key = drop_key(drop);
     if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
   }
-  const unsigned long long place = (unsigned long long)(w.r0 + r.ry) * p.C + c;
-  for (int t = 0;;) {
+  const unsigned long long place = (unsigned long long)l.ry * p.C + c;
+  for (;;) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (t + u >= r.steps) break;
+      if (u >= t.steps) break;
       float f[V];
       unpack<DT, V>(raw[u], f);
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
       act_fwd<V>(f, act);
       if (DROP) {
-        if (!drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, place + (unsigned long long)(t + u) * p.row_lanes * p.C);
+        if (!drop.per_channel)
+          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
         drop_apply<V>(f, keep, drop.scale);
       }
-      if (r.valid(t + u)) store_row(ys, t + u, f);
+      if (t.valid(u, l.ry)) ys.store(t, u, f);
     }
-    t += kU;
-    if (t >= r.steps) break;
-    xs.batch(r, t, raw);
+    if (t.index + p.chunks >= p.tiles) break;
+    t = Tile(p, t.index + p.chunks);
+    xs.load(t, l.ry, raw);
   }
 }
 
