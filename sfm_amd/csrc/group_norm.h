@@ -22,7 +22,17 @@ namespace sfm {
 namespace {
 
 
-constexpr int kTargetBlocks = 1024;  // four workgroups of four waves per CU: all of a launch is resident (2048 was two rounds of most kernels)
+// Workgroups per CU that a pass is launched with; a workgroup is one wave per SIMD, and all of a launch have to be resident (the
+// kernels' bounds hold their registers down to that): one more than fits is a second round of the whole length.  Measured at 0.5 GB
+// a tensor, us: statistics at 4 / 6 / 8: 97 / 94 / 98; forward's last pass fp32 at 4 / 6: 180 / 171, bf16 at 4 / 6: 193 / 200; backward's sums fp32 at 4 / 5: 194 / 172
+// (16-bit types hold two vectors of eight in registers: 4); its last pass fp32 at 4 / 5: 251 / 245.
+constexpr int kWavesStats = 6;
+constexpr int waves_apply(int es) { return es == 4 ? 6 : 4; }
+constexpr int waves_sums(int es) { return es == 4 ? 5 : 4; }
+constexpr int waves_bwd_apply(int es) { return es == 4 ? 5 : 4; }
+// (a vector that crosses many groups has a set of statistics for each and takes what registers it needs)
+constexpr int bound_of(int groups_of_vector, int waves) { return groups_of_vector <= 2 ? waves : 4; }
+constexpr int kCUs = 256;
 constexpr int kMaxChunks = 1024;
 constexpr int kU = 4;  // rows a thread has in flight
 
@@ -40,14 +50,16 @@ struct GnPlan {
   int parts;             // slabs of a group (1 where a slab holds whole groups)
   int lanes;             // cs / V
   int row_lanes;         // kBlock / lanes: rows a workgroup takes at once
-  int chunks;
-  int P;                 // partials of a group: chunks * parts
-  // rows into tiles and chunks (gn_tiles)
   int tile_rows;
   long long tiles;
-  long long own;         // tiles of a chunk; the first `extra` chunks have one more
-  int extra;
-  int owner, left;       // the chunk of the last tile, and the rows of that tile
+  int left;              // rows of the last tile
+  struct Turn {          // how a pass deals out the tiles
+    int chunks;
+    long long own;       // tiles of a chunk; the first `extra` chunks have one more
+    int extra;
+    int owner;           // the chunk of the last tile
+  } first, last;         // the pass that makes partial sums, and the one that joins and applies them
+  int P;                 // partials of a group: first.chunks * parts
 };
 
 static inline int gcd_int(int a, int b) {
@@ -55,20 +67,22 @@ static inline int gcd_int(int a, int b) {
   return a;
 }
 
-// (also after the number of chunks is known: a row stride may ask for fewer row lanes, which makes more tiles of the same chunks)
+// (also once the numbers of chunks are known: a row stride may ask for fewer row lanes, which makes more tiles of the same chunks)
 static void gn_tiles(GnPlan& p, int row_lanes) {
   p.row_lanes = row_lanes;
   p.tile_rows = kU * row_lanes;
   p.tiles = (p.N + p.tile_rows - 1) / p.tile_rows;
-  if (p.chunks < 1) p.chunks = 1;
-  p.own = p.tiles / p.chunks;
-  p.extra = (int)(p.tiles % p.chunks);
-  p.owner = (int)((p.tiles - 1) % p.chunks);
   p.left = (int)(p.N - (p.tiles - 1) * p.tile_rows);
+  for (GnPlan::Turn* t : {&p.first, &p.last}) {
+    if (t->chunks < 1) t->chunks = 1;
+    t->own = p.tiles / t->chunks;
+    t->extra = (int)(p.tiles % t->chunks);
+    t->owner = (int)((p.tiles - 1) % t->chunks);
+  }
 }
 
 // (the arguments have been checked; false: an item is too large)
-static bool gn_plan(long long B, long long N, int C, int G, int es, GnPlan& p) {
+static bool gn_plan(long long B, long long N, int C, int G, int es, bool backward, GnPlan& p) {
   p = GnPlan{};
   p.N = N; p.C = C; p.G = G; p.cpg = C / G;
   p.V = 16 / es;
@@ -100,11 +114,15 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, GnPlan& p) {
   }
   p.lanes = p.cs / p.V;
   gn_tiles(p, kBlock / p.lanes);
-  const long long per = (long long)B * p.slabs;
-  long long chunks = std::min({(kTargetBlocks + per - 1) / per, p.tiles, (long long)kMaxChunks});
-  const long long each = (p.tiles + chunks - 1) / chunks;  // as even as whole tiles allow
-  p.chunks = (int)((p.tiles + each - 1) / each);
-  p.P = p.chunks * p.parts;
+  auto deal = [&](int waves) {
+    const long long per = (long long)B * p.slabs;
+    const long long chunks = std::min({((long long)waves * kCUs + per - 1) / per, p.tiles, (long long)kMaxChunks});
+    const long long each = (p.tiles + chunks - 1) / chunks;  // as even as whole tiles allow
+    return (int)((p.tiles + each - 1) / each);
+  };
+  p.first.chunks = deal(backward ? waves_sums(es) : kWavesStats);
+  p.last.chunks = deal(backward ? waves_bwd_apply(es) : waves_apply(es));
+  p.P = p.first.chunks * p.parts;
   gn_tiles(p, p.row_lanes);
   return true;
 }
@@ -114,10 +132,10 @@ struct Where {
   int b, slab, chunk, part;
   int c0, cc, g0, ng;  // first channel and channels of the slab, first group and groups of it
 };
-__device__ __forceinline__ Where where(const GnPlan& p, unsigned bid) {
+__device__ __forceinline__ Where where(const GnPlan& p, int chunks, unsigned bid) {
   Where w;
-  w.chunk = bid % (unsigned)p.chunks;
-  bid /= (unsigned)p.chunks;
+  w.chunk = bid % (unsigned)chunks;
+  bid /= (unsigned)chunks;
   w.slab = bid % (unsigned)p.slabs;
   w.b = bid / (unsigned)p.slabs;
   if (p.parts == 1) {
@@ -161,7 +179,14 @@ struct Tile {
   __device__ __forceinline__ bool valid(int u, int ry) const { return full || u < steps - 1 || (u == steps - 1 && ry < last); }
 };
 
-template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, for tensors that no cache holds until they are read again (far(), below)
+// The last pass goes through a workgroup's tiles from the last one down: the first pass has left the latest of them in the caches
+// (the same workgroup on the same XCD, whose L2 is its own).  54 MB a tensor: 87.1 -> 83.8 us for the four passes; 0.5 GB a
+// tensor: 768 -> 784, so not there (FAR).
+__device__ __forceinline__ long long last_tile(const GnPlan& p, const Where& w) {
+  return w.chunk + (p.last.own + (w.chunk < p.last.extra) - 1) * p.last.chunks;
+}
+
+template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, for tensors that no cache holds until they are read again (far())
   static constexpr int kES = ElemBytes<DT>::value;
   const char* base;
   long long step;      // bytes of the rows of a step
@@ -172,24 +197,19 @@ template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, f
     lead = (unsigned)(l.ry * ld * kES);
     off = lead + (unsigned)(l.vx * V * kES);
   }
-  __device__ __forceinline__ const char* at(const Tile& t, int u) const { return base + (t.index * kU + u) * step; }
-  // one row of the tile, u < steps; in its last step a row lane without a row reads row lane 0's
-  __device__ __forceinline__ Raw<DT, V> row(const Tile& t, int u, int ry) const {
-    return load_raw<DT, V, NT>(at(t, u), off - (t.valid(u, ry) ? 0u : lead));
+  __device__ __forceinline__ const char* at(const Tile& t) const { return base + t.index * kU * step; }
+  // step u < steps of the tile at `a`; in its last step a row lane without a row reads row lane 0's
+  __device__ __forceinline__ Raw<DT, V> row(const char* a, const Tile& t, int u, int ry) const {
+    return load_raw<DT, V, NT>(a + u * step, off - (t.valid(u, ry) ? 0u : lead));
   }
   __device__ __forceinline__ void load(const Tile& t, int ry, Raw<DT, V> (&raw)[kU]) const {
-    if (t.full) {
-      const char* a = at(t, 0);
+    const char* a = at(t);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) { raw[u] = load_raw<DT, V, NT>(a, off); a += step; }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kU; ++u)
-        if (u < t.steps) raw[u] = row(t, u, ry);
-    }
+    for (int u = 0; u < kU; ++u)
+      if (u < t.steps) raw[u] = row(a, t, u, ry);
   }
-  __device__ __forceinline__ void store(const Tile& t, int u, const float (&f)[V]) const {
-    store_vec<DT, V, NT>(const_cast<char*>(at(t, u)), off, f);
+  __device__ __forceinline__ void store(const char* a, int u, const float (&f)[V]) const {
+    store_vec<DT, V, NT>(const_cast<char*>(a) + u * step, off, f);
   }
 };
 
@@ -208,21 +228,25 @@ template <typename F> __device__ __forceinline__ F team_sum(F v, int T) {
 // values that partial q of a group covers
 __device__ __forceinline__ double part_count(const GnPlan& p, int q) {
   const int chunk = p.parts == 1 ? q : q / p.parts, part = q - chunk * p.parts;
-  const double rows = (double)((p.own + (chunk < p.extra)) * p.tile_rows - (chunk == p.owner ? p.tile_rows - p.left : 0));
+  const double rows = (double)((p.first.own + (chunk < p.first.extra)) * p.tile_rows - (chunk == p.first.owner ? p.tile_rows - p.left : 0));
   return rows * (p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
 }
 
-// dispatch on the type, the vector width and whether a vector lies in one group: fn(DT, V, ONE) as integral constants
+// dispatch on the type, the vector width, and how many adjacent channels of a vector are of one group (a power of two that divides
+// both: a thread keeps one set of statistics for them): fn(DT, V, E) as integral constants
 template <typename F> static void by_type(int dtype, const GnPlan& p, F&& fn) {
   using std::integral_constant;
-  const bool one = p.cpg % p.V == 0;
+  int one = p.V;
+  while (p.cpg % one) one /= 2;
   auto width = [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
     auto go = [&](auto v) {
-      if (one) fn(dt, v, std::true_type{});
-      else if constexpr (decltype(v)::value > 1) fn(dt, v, std::false_type{});
+      constexpr int V = decltype(v)::value;
+      if constexpr (V >= 8) { if (one == 8) return fn(dt, v, integral_constant<int, 8>{}); }
+      if constexpr (V >= 4) { if (one == 4) return fn(dt, v, integral_constant<int, 4>{}); }
+      if constexpr (V >= 2) { if (one == 2) return fn(dt, v, integral_constant<int, 2>{}); }
+      fn(dt, v, integral_constant<int, 1>{});
     };
-    if constexpr (DT != kF32) { if (p.V == 8) return go(integral_constant<int, 8>{}); }
+    if constexpr (decltype(dt)::value != kF32) { if (p.V == 8) return go(integral_constant<int, 8>{}); }
     if (p.V == 4) return go(integral_constant<int, 4>{});
     if (p.V == 2) return go(integral_constant<int, 2>{});
     go(integral_constant<int, 1>{});
@@ -242,26 +266,23 @@ template <int DT, int V, typename F> static void by_use(bool drop, bool away, F&
   else fn(std::false_type{}, std::false_type{});
 }
 
-// The last pass over tensors that together pass the memory-side cache (256 MB) reads and writes nontemporally: nothing of them would be found
-// there again.  1024x2048x32 bf16 serve 650 -> 605 us, train 863 -> 778; under it a reader of the result may still find it, and
-// the pass itself gains little (concat4 of the 128x416 decoder, 54 MB a tensor: 87.1 -> 84.5 us for four passes).
-static inline bool far(long long bytes) { return bytes > (256ll << 20); }
-
 // rows of C elements of es bytes, ld elements apart
 static bool rows_ok(const void* q, long long ld, int C, int es) { return q && ld >= C && ((uintptr_t)q & (es - 1)) == 0; }
 
 // ld: the widest row stride of the call
-static int gn_setup(long long B, long long N, int C, int G, int dtype, long long ld, GnPlan& p, unsigned& grid) {
+static int gn_setup(long long B, long long N, int C, int G, int dtype, long long ld, bool backward, GnPlan& p, unsigned& first,
+                    unsigned& last) {
   if (dtype < kF32 || dtype > kF16 || B < 1 || N < 1 || C < 1 || G < 1 || C % G || ld < C) return SFM_ERR_ARG;
   const int es = dtype == kF32 ? 4 : 2;
   // items are counted in 32 bits, workgroups in 31, elements in 60 with room for strides; the rows that a workgroup takes at once
   // lie within 31 bits of bytes of each other
-  if (B > 0x7fffffffll || (__int128)B * N > ((__int128)1 << 40) || ld > 0x7fffffffll / es || !gn_plan(B, N, C, G, es, p))
+  if (B > 0x7fffffffll || (__int128)B * N > ((__int128)1 << 40) || ld > 0x7fffffffll / es || !gn_plan(B, N, C, G, es, backward, p))
     return SFM_ERR_TOO_LARGE;
   gn_tiles(p, (int)std::min<long long>(p.row_lanes, 0x7fffffffll / (ld * es)));
-  const __int128 blocks = (__int128)B * p.slabs * p.chunks;
-  if (blocks + C > 0x7fffffffll) return SFM_ERR_TOO_LARGE;
-  grid = (unsigned)blocks;
+  const __int128 blocks = (__int128)B * p.slabs * std::max(p.first.chunks, p.last.chunks);
+  if (blocks + C > 0x7fffffffll) return SFM_ERR_TOO_LARGE;  // (with those that sum the parameters' gradients)
+  first = (unsigned)(B * p.slabs * p.first.chunks);
+  last = (unsigned)(B * p.slabs * p.last.chunks);
   return SFM_OK;
 }
 

@@ -17,22 +17,22 @@ __device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, con
   for (int k = 1; k < s.n; ++k) {  // uniform
     const Stream<DT, V> more(s.p[k], s.ld[k], p, w, l);
     float f[V];
-    unpack<DT, V>(more.row(t, u, l.ry), f);
+    unpack<DT, V>(more.row(more.at(t), t, u, l.ry), f);
 #pragma unroll
     for (int e = 0; e < V; ++e) g[e] += f[e];
   }
 }
 
 // ---- backward, first launch: per_group [B][G][P] (sum gamma dz, sum gamma dz xhat), per_channel [C][B][chunks] (sum dz, sum dz xhat)
-template <int DT, int V, bool ONE, bool DROP>
-__global__ __launch_bounds__(kBlock, 4) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+template <int DT, int V, int E, bool DROP>
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::value))) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                              const float* __restrict__ gamma, const float* __restrict__ beta,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
                                                              GnPlan p, int B, int act, Drop drop, float2* __restrict__ per_group,
                                                              float2* __restrict__ per_channel) {
-  constexpr int A = ONE ? 1 : V, E = V / A;
+  constexpr int A = V / E;
   __shared__ float2 red[kBlock * V];
-  const Where w = where(p, blockIdx.x);
+  const Where w = where(p, p.first.chunks, blockIdx.x);
   const Lane l(p, w);
   if (l.mine) {
     const Stream<DT, V> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l);
@@ -75,8 +75,8 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_sums_kernel(const void* __re
 #pragma unroll
         for (int k = 0; k < V; ++k) { s1[k] += g[k]; s2[k] = __builtin_fmaf(g[k], f[k], s2[k]); }
       }
-      if (t.index + p.chunks >= p.tiles) break;
-      t = Tile(p, t.index + p.chunks);
+      if (t.index + p.first.chunks >= p.tiles) break;
+      t = Tile(p, t.index + p.first.chunks);
       xs.load(t, l.ry, xr);
       gs.load(t, l.ry, gr);
     }
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_sums_kernel(const void* __re
     float2 v = red[c];
     for (int i = 1; i < left; ++i) { const float2 o = red[i * p.cs + c]; v.x += o.x; v.y += o.y; }
     red[c] = v;
-    per_channel[((long long)(w.c0 + c) * B + w.b) * p.chunks + w.chunk] = v;
+    per_channel[((long long)(w.c0 + c) * B + w.b) * p.first.chunks + w.chunk] = v;
   }
   __syncthreads();
   const Team tm = team_of(w.ng);
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_sums_kernel(const void* __re
 
 // ---- backward, second launch: the first param_blocks workgroups sum the channel partials over items and chunks (a wave per
 // channel), the others write gx
-template <int DT, int V, bool ONE, bool DROP, bool FAR>
-__global__ __launch_bounds__(kBlock, 4) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+template <int DT, int V, int E, bool DROP, bool FAR>
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<DT>::value))) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
                                                               GnPlan p, int B, int act, Drop drop,
@@ -128,12 +128,12 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_apply_kernel(const void* __r
                                                               const float2* __restrict__ per_channel, unsigned param_blocks,
                                                               void* __restrict__ gx, float* __restrict__ ggamma,
                                                               float* __restrict__ gbeta) {
-  constexpr int A = ONE ? 1 : V, E = V / A;
+  constexpr int A = V / E;
   __shared__ float2 stat[kBlock * A];
   if (blockIdx.x < param_blocks) {
     const int c = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (c >= p.C) return;
-    const long long n = (long long)B * p.chunks;
+    const long long n = (long long)B * p.first.chunks;
     const float2* src = per_channel + c * n;
     double a = 0.0, b = 0.0;
     for (long long k = lane; k < n; k += 64) { const float2 v = src[k]; a += v.x; b += v.y; }
@@ -142,10 +142,10 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_apply_kernel(const void* __r
     if (lane == 0) { gbeta[c] = (float)a; ggamma[c] = (float)b; }
     return;
   }
-  const Where w = where(p, blockIdx.x - param_blocks);
+  const Where w = where(p, p.last.chunks, blockIdx.x - param_blocks);
   const Lane l(p, w);
   const Stream<DT, V, FAR> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l), os(gx, p.C, p, w, l);
-  Tile t(p, w.chunk);
+  Tile t(p, FAR ? w.chunk : last_tile(p, w));
   Raw<DT, V> xr[kU], gr[kU];
   const int c = w.c0 + l.vx * V;
   float mu[A], is[A], ga[V], be[V], c1[A], c2[A];
@@ -188,6 +188,7 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_apply_kernel(const void* __r
   }
   const unsigned long long place = (unsigned long long)l.ry * p.C + c;
   for (;;) {
+    const char* o = os.at(t);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       if (u >= t.steps) break;
@@ -206,10 +207,10 @@ __global__ __launch_bounds__(kBlock, 4) void gn_bwd_apply_kernel(const void* __r
 #pragma unroll
       for (int k = 0; k < V; ++k)
         g[k] = is[k / E] * __builtin_fmaf(-f[k], c2[k / E], __builtin_fmaf(ga[k], g[k], -c1[k / E]));
-      if (t.valid(u, l.ry)) os.store(t, u, g);
+      if (t.valid(u, l.ry)) os.store(o, u, g);
     }
-    if (t.index + p.chunks >= p.tiles) break;
-    t = Tile(p, t.index + p.chunks);
+    if (FAR ? t.index + p.last.chunks >= p.tiles : t.index < p.last.chunks) break;
+    t = Tile(p, FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
     xs.load(t, l.ry, xr);
     gs.load(t, l.ry, gr);
   }
@@ -227,12 +228,12 @@ extern "C" int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, 
                                       int per_channel, void* gx, float* ggamma, float* gbeta, float* ws, void* stream_) {
   GnPlan p;
   Drop d;
-  unsigned grid;
+  unsigned first, last;
   const int es = dtype == kF32 ? 4 : 2;
   if (!gy || !ld_gy || n_gy < 1 || n_gy > 3) return SFM_ERR_ARG;
   long long ld = ld_x;
   for (int k = 0; k < n_gy; ++k) ld = std::max(ld, ld_gy[k]);
-  const int rc = gn_setup(B, N, C, G, dtype, ld, p, grid);
+  const int rc = gn_setup(B, N, C, G, dtype, ld, true, p, first, last);
   if (rc) return rc;
   if (!rows_ok(x, ld_x, C, es) || !gamma || !beta || !save_mean || !save_rstd ||
       (!gx && !ggamma) || (gx && !rows_ok(gx, C, C, es)) || (!ggamma != !gbeta) || !ws || ((uintptr_t)ws & 7) || act < kActNone ||
@@ -249,16 +250,17 @@ extern "C" int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, 
   hipStream_t stream = (hipStream_t)stream_;
   float2* per_group = reinterpret_cast<float2*>(ws);
   float2* per_channel_sums = per_group + B * G * p.P;
-  const unsigned params = ggamma ? (unsigned)((C + kBlock / 64 - 1) / (kBlock / 64)) : 0u;
-  const unsigned second = params + (gx ? grid : 0u);
-  by_type(dtype, p, [&](auto dt, auto v, auto one) {
+  // a multiple of eight: the workgroups behind them stay on the XCDs they were on in the first launch
+  const unsigned params = ggamma ? ((unsigned)(C + kBlock / 64 - 1) / (kBlock / 64) + 7u) / 8u * 8u : 0u;
+  const unsigned second = params + (gx ? last : 0u);
+  by_type(dtype, p, [&](auto dt, auto v, auto e) {
     constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
-    constexpr bool ONE = decltype(one)::value;
+    constexpr int E = decltype(e)::value;
     by_use<DT, V>(threshold != 0, far(3 * B * N * C * es), [&](auto drop, auto away) {
       constexpr bool DROP = decltype(drop)::value;
-      hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, ONE, DROP>), dim3(grid), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta, save_mean,
+      hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, E, DROP>), dim3(first), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta, save_mean,
                          save_rstd, p, (int)B, act, d, per_group, per_channel_sums);
-      hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, ONE, DROP, decltype(away)::value>), dim3(second), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta,
+      hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, E, DROP, decltype(away)::value>), dim3(second), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta,
                          save_mean, save_rstd, p, (int)B, act, d, per_group, per_channel_sums, params, gx, ggamma, gbeta);
     });
   });

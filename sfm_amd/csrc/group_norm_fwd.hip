@@ -4,14 +4,13 @@
 namespace sfm {
 namespace {
 
-// ---- forward, first launch: part [B][G][P] (mean, M2).  ONE: the V channels of a vector are of one group (V divides cpg), and a
-// thread has one pair for them; else one pair per channel.
-template <int DT, int V, bool ONE>
-__global__ __launch_bounds__(kBlock, 4) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
+// ---- forward, first launch: part [B][G][P] (mean, M2).  A thread has one pair for E adjacent channels of a group.
+template <int DT, int V, int E>
+__global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
                                                           float2* __restrict__ part) {
-  constexpr int A = ONE ? 1 : V, E = V / A;  // accumulators, and elements of one in a row
-  __shared__ float2 red[kBlock * A];         // [row lane][vector or channel of the slab]
-  const Where w = where(p, blockIdx.x);
+  constexpr int A = V / E;                   // accumulators
+  __shared__ float2 red[kBlock * A];         // [row lane][E channels of the slab]
+  const Where w = where(p, p.first.chunks, blockIdx.x);
   const Lane l(p, w);
   if (l.mine) {
     const Stream<DT, V> xs(x, ldx, p, w, l);
@@ -49,7 +48,7 @@ __global__ __launch_bounds__(kBlock, 4) void gn_stats_kernel(const void* __restr
       }
       n = nn;
     };
-    for (long long i = w.chunk; i < p.tiles; i += p.chunks) {
+    for (long long i = w.chunk; i < p.tiles; i += p.first.chunks) {
       const Tile t(p, i);
       Raw<DT, V> raw[kU];
       xs.load(t, l.ry, raw);
@@ -57,7 +56,7 @@ __global__ __launch_bounds__(kBlock, 4) void gn_stats_kernel(const void* __restr
       else {
 #pragma unroll
         for (int u = 0; u < kU; ++u)
-          if (u < t.steps && t.valid(u, l.ry)) join(std::integral_constant<int, 1>{}, raw + u);
+          if (t.valid(u, l.ry)) join(std::integral_constant<int, 1>{}, raw + u);
       }
     }
 #pragma unroll
@@ -67,8 +66,8 @@ __global__ __launch_bounds__(kBlock, 4) void gn_stats_kernel(const void* __restr
   // over the row lanes and the vectors of a group.  Means are taken against one of them, so a common part costs no digits.
   const Team tm = team_of(w.ng);
   const int per_row = (p.parts == 1 ? p.cpg : w.cc) / E;           // pairs of a group in a row lane
-  const bool partial = w.chunk == p.owner && p.left < p.tile_rows;
-  const long long whole = p.own + (w.chunk < p.extra) - partial;   // whole tiles of this chunk
+  const bool partial = w.chunk == p.first.owner && p.left < p.tile_rows;
+  const long long whole = p.first.own + (w.chunk < p.first.extra) - partial;   // whole tiles of this chunk
   const int tail = partial ? p.left / p.row_lanes : 0, more = partial ? p.left % p.row_lanes : 0;
   const float rows = (float)(whole * kU + tail);                   // of a row lane; the first `more` lanes have one more
   const int busy = whole > 0 || tail > 0 ? p.row_lanes : more;     // row lanes that have seen a row
@@ -116,19 +115,20 @@ __device__ __forceinline__ void join_stats(const float2* __restrict__ part, cons
   __syncthreads();
 }
 
-// ---- forward, second launch.  The first batch is on its way while the partials are joined.
-template <int DT, int V, bool ONE, bool DROP, bool FAR>
-__global__ __launch_bounds__(kBlock, 4) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
+// ---- forward, second launch.  The first batch is on its way while the partials are joined; where a cache may still hold what the
+// first launch read last, the tiles go backwards (last_tile).
+template <int DT, int V, int E, bool DROP, bool FAR>
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::value))) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
                                                           const float2* __restrict__ part, GnPlan p, float eps, int act, Drop drop,
                                                           void* __restrict__ y, long long ldy, float* __restrict__ save_mean,
                                                           float* __restrict__ save_r) {
-  constexpr int A = ONE ? 1 : V, E = V / A;
+  constexpr int A = V / E;
   __shared__ float2 stat[kBlock * A];
-  const Where w = where(p, blockIdx.x);
+  const Where w = where(p, p.last.chunks, blockIdx.x);
   const Lane l(p, w);
   const Stream<DT, V, FAR> xs(x, ldx, p, w, l), ys(y, ldy, p, w, l);
-  Tile t(p, w.chunk);
+  Tile t(p, FAR ? w.chunk : last_tile(p, w));
   Raw<DT, V> raw[kU];
   float sc[V], sh[V];
   const int c = w.c0 + l.vx * V;
@@ -160,11 +160,15 @@ __global__ __launch_bounds__(kBlock, 4) void gn_apply_kernel(const void* __restr
   }
   const unsigned long long place = (unsigned long long)l.ry * p.C + c;
   for (;;) {
+    const bool more = FAR ? t.index + p.last.chunks < p.tiles : t.index >= p.last.chunks;
+    const Tile next(p, !more ? t.index : FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
+    const char *a = xs.at(next), *o = ys.at(t);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       if (u >= t.steps) break;
       float f[V];
       unpack<DT, V>(raw[u], f);
+      if (more && u < next.steps) raw[u] = xs.row(a, next, u, l.ry);  // as a row has been used, the next tile's is asked for
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
       act_fwd<V>(f, act);
@@ -173,11 +177,10 @@ __global__ __launch_bounds__(kBlock, 4) void gn_apply_kernel(const void* __restr
           keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
         drop_apply<V>(f, keep, drop.scale);
       }
-      if (t.valid(u, l.ry)) ys.store(t, u, f);
+      if (t.valid(u, l.ry)) ys.store(o, u, f);
     }
-    if (t.index + p.chunks >= p.tiles) break;
-    t = Tile(p, t.index + p.chunks);
-    xs.load(t, l.ry, raw);
+    if (!more) break;
+    t = next;
   }
 }
 
@@ -188,10 +191,10 @@ using namespace sfm;
 
 extern "C" long long sfm_group_norm_workspace_floats(long long B, long long N, int C, int G, int dtype, int backward) {
   GnPlan p;
-  unsigned grid;
-  const int rc = gn_setup(B, N, C, G, dtype, C, p, grid);
+  unsigned first, last;
+  const int rc = gn_setup(B, N, C, G, dtype, C, backward != 0, p, first, last);
   if (rc) return rc;
-  return 2 * (B * G * p.P + (backward ? B * C * p.chunks : 0));
+  return 2 * (B * G * p.P + (backward ? B * C * p.first.chunks : 0));
 }
 
 extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, const float* gamma, const float* beta, long long B,
@@ -200,9 +203,9 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
                                       long long ld_y, float* save_mean, float* save_rstd, float* ws, void* stream_) {
   GnPlan p;
   Drop d;
-  unsigned grid;
+  unsigned first, last;
   const int es = dtype == kF32 ? 4 : 2;
-  const int rc = gn_setup(B, N, C, G, dtype, std::max(ld_x, ld_y), p, grid);
+  const int rc = gn_setup(B, N, C, G, dtype, std::max(ld_x, ld_y), false, p, first, last);
   if (rc) return rc;
   if (!rows_ok(x, ld_x, C, es) || !rows_ok(y, ld_y, C, es) || !gamma || !beta || !ws || ((uintptr_t)ws & 7) || !(eps > 0.0f) ||
       act < kActNone || act > kActSilu || (!save_mean != !save_rstd) ||
@@ -211,12 +214,12 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
   if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > 0xffffffffll - item0)) return SFM_ERR_TOO_LARGE;
   hipStream_t stream = (hipStream_t)stream_;
   float2* part = reinterpret_cast<float2*>(ws);
-  by_type(dtype, p, [&](auto dt, auto v, auto one) {
+  by_type(dtype, p, [&](auto dt, auto v, auto e) {
     constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
-    constexpr bool ONE = decltype(one)::value;
-    hipLaunchKernelGGL((gn_stats_kernel<DT, V, ONE>), dim3(grid), dim3(kBlock), 0, stream, x, ld_x, p, part);
+    constexpr int E = decltype(e)::value;
     by_use<DT, V>(threshold != 0, far(2 * B * N * C * es), [&](auto drop, auto away) {
-      hipLaunchKernelGGL((gn_apply_kernel<DT, V, ONE, decltype(drop)::value, decltype(away)::value>), dim3(grid), dim3(kBlock), 0, stream,
+      hipLaunchKernelGGL((gn_stats_kernel<DT, V, E>), dim3(first), dim3(kBlock), 0, stream, x, ld_x, p, part);
+      hipLaunchKernelGGL((gn_apply_kernel<DT, V, E, decltype(drop)::value, decltype(away)::value>), dim3(last), dim3(kBlock), 0, stream,
                          x, ld_x, gamma, beta, part, p, eps, act, d, y, ld_y, save_mean, save_rstd);
     });
   });
