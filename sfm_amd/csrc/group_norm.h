@@ -215,10 +215,10 @@ template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, f
 
 // Teams: the workgroup's threads, cut into teams of T lanes of one wave (T a power of two), one group each at a time.
 struct Team { int T, id, lane, count; };
-__device__ __forceinline__ Team team_of(int ng) {
+template <int THREADS = kBlock> __device__ __forceinline__ Team team_of(int ng) {
   int T = 64;
-  while (T > 1 && kBlock / T < ng) T >>= 1;
-  return {T, (int)threadIdx.x / T, (int)threadIdx.x & (T - 1), kBlock / T};
+  while (T > 1 && THREADS / T < ng) T >>= 1;
+  return {T, (int)threadIdx.x / T, (int)threadIdx.x & (T - 1), THREADS / T};
 }
 template <typename F> __device__ __forceinline__ F team_sum(F v, int T) {
   for (int o = T >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

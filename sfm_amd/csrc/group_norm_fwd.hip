@@ -4,6 +4,34 @@
 namespace sfm {
 namespace {
 
+// (mean, M2) of the groups of a workgroup from those of its threads: red [row lane][vector][A], a pair for each E adjacent channels of
+// a vector.  Every row lane has seen per_lane rows, the first `more` one more.  cg: channels of a group in the slab.  Means are
+// taken against one of them, so a common part costs no digits.  out(j, mean, M2) by one thread per group.
+template <int T, int A, int E, typename F>
+__device__ __forceinline__ void reduce_stats(const float2* red, int lanes, int row_lanes, int per_lane, int more, int cg, int ng, F&& out) {
+  const Team tm = team_of<T>(ng);
+  const int per_row = cg / E, busy = per_lane > 0 ? row_lanes : more;
+  const float rows = (float)per_lane, inv = 1.0f / ((rows * row_lanes + more) * per_row);
+  for (int j = tm.id; j < ng; j += tm.count) {
+    const float ref = red[j * per_row].x;
+    float s = 0.0f;
+    for (int e = tm.lane; e < busy * per_row; e += tm.T) {
+      const int row = e / per_row, c = e - row * per_row;
+      s = __builtin_fmaf(rows + (row < more), red[row * lanes * A + j * per_row + c].x - ref, s);
+    }
+    const float off = team_sum(s, tm.T) * inv;
+    float q = 0.0f;
+    for (int e = tm.lane; e < busy * per_row; e += tm.T) {
+      const int row = e / per_row, c = e - row * per_row;
+      const float2 v = red[row * lanes * A + j * per_row + c];
+      const float d = (v.x - ref) - off;
+      q += __builtin_fmaf(E * (rows + (row < more)) * d, d, v.y);
+    }
+    q = team_sum(q, tm.T);
+    if (tm.lane == 0) out(j, ref + off, q);
+  }
+}
+
 // ---- forward, first launch: part [B][G][P] (mean, M2).  A thread has one pair for E adjacent channels of a group.
 template <int DT, int V, int E>
 __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
@@ -63,33 +91,12 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats
     for (int a = 0; a < A; ++a) red[(l.ry * p.lanes + l.vx) * A + a] = make_float2(mean[a], m2[a]);
   }
   __syncthreads();
-  // over the row lanes and the vectors of a group.  Means are taken against one of them, so a common part costs no digits.
-  const Team tm = team_of(w.ng);
-  const int per_row = (p.parts == 1 ? p.cpg : w.cc) / E;           // pairs of a group in a row lane
   const bool partial = w.chunk == p.first.owner && p.left < p.tile_rows;
   const long long whole = p.first.own + (w.chunk < p.first.extra) - partial;   // whole tiles of this chunk
-  const int tail = partial ? p.left / p.row_lanes : 0, more = partial ? p.left % p.row_lanes : 0;
-  const float rows = (float)(whole * kU + tail);                   // of a row lane; the first `more` lanes have one more
-  const int busy = whole > 0 || tail > 0 ? p.row_lanes : more;     // row lanes that have seen a row
-  const float inv = 1.0f / ((rows * p.row_lanes + more) * per_row);
-  for (int j = tm.id; j < w.ng; j += tm.count) {
-    const float ref = red[j * per_row].x;
-    float s = 0.0f;
-    for (int e = tm.lane; e < busy * per_row; e += tm.T) {
-      const int row = e / per_row, c = e - row * per_row;
-      s = __builtin_fmaf(rows + (row < more), red[row * p.lanes * A + j * per_row + c].x - ref, s);
-    }
-    const float off = team_sum(s, tm.T) * inv;
-    float q = 0.0f;
-    for (int e = tm.lane; e < busy * per_row; e += tm.T) {
-      const int row = e / per_row, c = e - row * per_row;
-      const float2 v = red[row * p.lanes * A + j * per_row + c];
-      const float d = (v.x - ref) - off;
-      q += __builtin_fmaf(E * (rows + (row < more)) * d, d, v.y);
-    }
-    q = team_sum(q, tm.T);
-    if (tm.lane == 0) part[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(ref + off, q);
-  }
+  const int per_lane = (int)whole * kU + (partial ? p.left / p.row_lanes : 0), more = partial ? p.left % p.row_lanes : 0;
+  reduce_stats<kBlock, A, E>(red, p.lanes, p.row_lanes, per_lane, more, p.parts == 1 ? p.cpg : w.cc, w.ng, [&](int j, float mean, float m2) {
+    part[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(mean, m2);
+  });
 }
 
 // joins the partials of a workgroup's groups: stat[j] = (mean, r) in LDS.  All threads call it; it ends with a barrier.
@@ -184,6 +191,111 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
   }
 }
 
+// ---- forward in one launch, for an item whose slab fits a workgroup's registers: a thread keeps up to kHeld vectors, the statistics
+// are the workgroup's own, x is read once.  The row lanes are T / lanes, whatever the plan of the two-launch form says.
+constexpr int kHeld = 4;
+
+template <int DT, int V, int E, bool DROP, int T>
+__global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, long long ldx, const float* __restrict__ gamma,
+                                                    const float* __restrict__ beta, GnPlan p, float eps, int act, Drop drop,
+                                                    void* __restrict__ y, long long ldy, float* __restrict__ save_mean,
+                                                    float* __restrict__ save_r) {
+  constexpr int A = V / E, kES = ElemBytes<DT>::value;
+  __shared__ float2 red[T * A], stat[T * A];
+  const Where w = where(p, 1, blockIdx.x);
+  const int N = (int)p.N, row_lanes = T / p.lanes;
+  const int vx = threadIdx.x % (unsigned)p.lanes, ry = threadIdx.x / (unsigned)p.lanes;
+  const bool mine = ry < row_lanes && vx * V < w.cc;
+  const int per_lane = N / row_lanes, more = N % row_lanes;
+  const int rows = mine ? per_lane + (ry < more) : 0;  // of this thread
+  const int c = w.c0 + vx * V;
+  const char* xs = static_cast<const char*>(x) + ((long long)w.b * N * ldx + c) * kES + ry * ldx * kES;
+  Raw<DT, V> raw[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (u < rows) raw[u] = load_raw<DT, V>(xs, (long long)u * row_lanes * ldx * kES);
+  float sc[V], sh[V];
+  if (mine) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k]; sh[k] = beta[c + k]; }
+    float s[A], q[A];
+#pragma unroll
+    for (int a = 0; a < A; ++a) { s[a] = 0.0f; q[a] = 0.0f; }
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (u < rows) {
+        float f[V];
+        unpack<DT, V>(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[k / E] += f[k];
+      }
+    const float share = rows ? 1.0f / (float)(rows * E) : 0.0f;
+#pragma unroll
+    for (int a = 0; a < A; ++a) s[a] *= share;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (u < rows) {
+        float f[V];
+        unpack<DT, V>(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) { const float d = f[k] - s[k / E]; q[k / E] = __builtin_fmaf(d, d, q[k / E]); }
+      }
+#pragma unroll
+    for (int a = 0; a < A; ++a) red[(ry * p.lanes + vx) * A + a] = make_float2(s[a], q[a]);
+  }
+  __syncthreads();
+  const float inv = 1.0f / ((float)N * (float)p.cpg);
+  reduce_stats<T, A, E>(red, p.lanes, row_lanes, per_lane, more, p.cpg, w.ng, [&](int j, float mean, float m2) {
+    const float r = 1.0f / sqrtf(__builtin_fmaf(m2, inv, eps));
+    stat[j] = make_float2(mean, r);
+    if (save_mean) {
+      save_mean[(long long)w.b * p.G + w.g0 + j] = mean;
+      save_r[(long long)w.b * p.G + w.g0 + j] = r;
+    }
+  });
+  __syncthreads();
+  if (!mine) return;
+  float mu[A];
+#pragma unroll
+  for (int a = 0; a < A; ++a) {
+    const float2 st = stat[(c + a * E) / p.cpg - w.g0];
+    mu[a] = st.x;
+#pragma unroll
+    for (int k = a * E; k < (a + 1) * E; ++k) sc[k] *= st.y;
+  }
+  DropKey key{};
+  unsigned keep = 0;
+  if (DROP) {
+    key = drop_key(drop);
+    if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
+  }
+  char* ys = static_cast<char*>(y) + ((long long)w.b * N * ldy + c) * kES + ry * ldy * kES;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    if (u < rows) {
+      float f[V];
+      unpack<DT, V>(raw[u], f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
+      act_fwd<V>(f, act);
+      if (DROP) {
+        if (!drop.per_channel)
+          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(u * row_lanes + ry) * p.C + c);
+        drop_apply<V>(f, keep, drop.scale);
+      }
+      store_vec<DT, V>(ys, (long long)u * row_lanes * ldy * kES, f);
+    }
+  }
+}
+
+// threads of the one-launch form, or 0 where an item's slab does not fit it
+static int held_threads(const GnPlan& p, int es) {
+  if (p.parts != 1 || p.V * es != 16) return 0;
+  for (int T : {256, 1024})
+    if (p.N <= (long long)kHeld * (T / p.lanes)) return T;
+  return 0;
+}
+
 }  // namespace
 }  // namespace sfm
 
@@ -214,9 +326,21 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
   if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > 0xffffffffll - item0)) return SFM_ERR_TOO_LARGE;
   hipStream_t stream = (hipStream_t)stream_;
   float2* part = reinterpret_cast<float2*>(ws);
+  const int held = held_threads(p, es);
+  const unsigned slabs = (unsigned)(B * p.slabs);
   by_type(dtype, p, [&](auto dt, auto v, auto e) {
     constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
     constexpr int E = decltype(e)::value;
+    if constexpr (V * ElemBytes<DT>::value == 16) {
+      auto one = [&](auto threads, auto drop) {
+        constexpr int T = decltype(threads)::value;
+        hipLaunchKernelGGL((gn_held_kernel<DT, V, E, decltype(drop)::value, T>), dim3(slabs), dim3(T), 0, stream, x, ld_x, gamma, beta, p,
+                           eps, act, d, y, ld_y, save_mean, save_rstd);
+      };
+      auto with = [&](auto threads) { threshold ? one(threads, std::true_type{}) : one(threads, std::false_type{}); };
+      if (held == 256) return with(std::integral_constant<int, 256>{});
+      if (held == 1024) return with(std::integral_constant<int, 1024>{});
+    }
     by_use<DT, V>(threshold != 0, far(2 * B * N * C * es), [&](auto drop, auto away) {
       hipLaunchKernelGGL((gn_stats_kernel<DT, V, E>), dim3(first), dim3(kBlock), 0, stream, x, ld_x, p, part);
       hipLaunchKernelGGL((gn_apply_kernel<DT, V, E, decltype(drop)::value, decltype(away)::value>), dim3(last), dim3(kBlock), 0, stream,
