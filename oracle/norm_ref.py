@@ -74,6 +74,8 @@ def group_norm_act(x, gamma, beta, groups, eps, kind, gy=None, keep=None, thresh
         gx = rstd * (dg - dg.mean(axis=(1, 3), keepdims=True) - xhat * (dg * xhat).mean(axis=(1, 3), keepdims=True))
         out.update(gx=gx.reshape(x.shape), ggamma=(dz * xhat).sum(axis=(0, 1)).reshape(C), gbeta=dz.sum(axis=(0, 1)).reshape(C),
                    abs_ggamma=np.abs(dz * xhat).sum(axis=(0, 1)).reshape(C), abs_gbeta=np.abs(dz).sum(axis=(0, 1)).reshape(C),
+                   abs_gy=np.where(k > 0, scale * np.abs(np.asarray(gy, dtype=np.float64).reshape(v.shape)), 0.0).sum(axis=(0, 1)).reshape(C),
+                   xhat_max=np.abs(xhat).max(),
                    # the largest of each (item, group), broadcast: what an error of gx is measured against
                    gx_size=np.broadcast_to(rstd * np.abs(dg).max(axis=(1, 3), keepdims=True)
                                            * (1 + np.abs(xhat).max(axis=(1, 3), keepdims=True)) ** 2, v.shape).reshape(x.shape))

@@ -49,6 +49,7 @@ struct GnPlan {
   int groups_per_slab;   // >= 1; 1 where a group has parts
   int parts;             // slabs of a group (1 where a slab holds whole groups)
   int lanes;             // cs / V
+  unsigned lanes_inv, cpg_inv;  // ceil(2^20 / lanes), ceil(2^32 / cpg) (0: one channel per group): quotients by a product
   int row_lanes;         // kBlock / lanes: rows a workgroup takes at once
   int tile_rows;
   long long tiles;
@@ -113,6 +114,8 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, bool backwar
     p.slabs = G * p.parts;
   }
   p.lanes = p.cs / p.V;
+  p.lanes_inv = ((1u << 20) + p.lanes - 1) / p.lanes;
+  p.cpg_inv = p.cpg == 1 ? 0u : (unsigned)(((1ull << 32) + p.cpg - 1) / p.cpg);
   gn_tiles(p, kBlock / p.lanes);
   auto deal = [&](int waves) {
     const long long per = (long long)B * p.slabs;
@@ -132,12 +135,12 @@ struct Where {
   int b, slab, chunk, part;
   int c0, cc, g0, ng;  // first channel and channels of the slab, first group and groups of it
 };
-__device__ __forceinline__ Where where(const GnPlan& p, int chunks, unsigned bid) {
+// a grid is (items, chunks, slabs): with a multiple of eight items all of an item is on one XCD in every pass
+__device__ __forceinline__ Where where(const GnPlan& p, unsigned b, unsigned chunk, unsigned slab) {
   Where w;
-  w.chunk = bid % (unsigned)chunks;
-  bid /= (unsigned)chunks;
-  w.slab = bid % (unsigned)p.slabs;
-  w.b = bid / (unsigned)p.slabs;
+  w.b = b;
+  w.chunk = chunk;
+  w.slab = slab;
   if (p.parts == 1) {
     w.part = 0;
     w.g0 = w.slab * p.groups_per_slab;
@@ -160,12 +163,16 @@ __device__ __forceinline__ Where where(const GnPlan& p, int chunks, unsigned bid
 struct Lane {
   int vx, ry;
   bool mine;  // this thread has a vector at all
-  __device__ __forceinline__ Lane(const GnPlan& p, const Where& w) {
-    vx = threadIdx.x % (unsigned)p.lanes;
-    ry = threadIdx.x / (unsigned)p.lanes;
-    mine = ry < p.row_lanes && vx * p.V < w.cc;
+  __device__ __forceinline__ Lane(const GnPlan& p, const Where& w, int row_lanes) {
+    ry = threadIdx.x * p.lanes_inv >> 20;  // threadIdx.x / lanes: exact, 1024 * 256 < 2^20
+    vx = threadIdx.x - ry * p.lanes;
+    mine = ry < row_lanes && vx * p.V < w.cc;
   }
 };
+// the group of a slab's channel, in the slab: channel / cpg, exact, 2048 * 2048 < 2^32
+__device__ __forceinline__ int group_in_slab(const GnPlan& p, int channel) {
+  return p.parts > 1 ? 0 : p.cpg_inv ? (int)__umulhi((unsigned)channel, p.cpg_inv) : channel;
+}
 struct Tile {
   long long index;
   int steps;  // steps in which row lane 0 has a row
@@ -226,10 +233,10 @@ template <typename F> __device__ __forceinline__ F team_sum(F v, int T) {
 }
 
 // values that partial q of a group covers
-__device__ __forceinline__ double part_count(const GnPlan& p, int q) {
+__device__ __forceinline__ float part_count(const GnPlan& p, int q) {
   const int chunk = p.parts == 1 ? q : q / p.parts, part = q - chunk * p.parts;
-  const double rows = (double)((p.first.own + (chunk < p.first.extra)) * p.tile_rows - (chunk == p.first.owner ? p.tile_rows - p.left : 0));
-  return rows * (p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
+  const long long rows = (p.first.own + (chunk < p.first.extra)) * p.tile_rows - (chunk == p.first.owner ? p.tile_rows - p.left : 0);
+  return (float)rows * (float)(p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
 }
 
 // dispatch on the type, the vector width, and how many adjacent channels of a vector are of one group (a power of two that divides
@@ -270,8 +277,8 @@ template <int DT, int V, typename F> static void by_use(bool drop, bool away, F&
 static bool rows_ok(const void* q, long long ld, int C, int es) { return q && ld >= C && ((uintptr_t)q & (es - 1)) == 0; }
 
 // ld: the widest row stride of the call
-static int gn_setup(long long B, long long N, int C, int G, int dtype, long long ld, bool backward, GnPlan& p, unsigned& first,
-                    unsigned& last) {
+static int gn_setup(long long B, long long N, int C, int G, int dtype, long long ld, bool backward, GnPlan& p, dim3& first,
+                    dim3& last) {
   if (dtype < kF32 || dtype > kF16 || B < 1 || N < 1 || C < 1 || G < 1 || C % G || ld < C) return SFM_ERR_ARG;
   const int es = dtype == kF32 ? 4 : 2;
   // items are counted in 32 bits, workgroups in 31, elements in 60 with room for strides; the rows that a workgroup takes at once
@@ -280,9 +287,9 @@ static int gn_setup(long long B, long long N, int C, int G, int dtype, long long
     return SFM_ERR_TOO_LARGE;
   gn_tiles(p, (int)std::min<long long>(p.row_lanes, 0x7fffffffll / (ld * es)));
   const __int128 blocks = (__int128)B * p.slabs * std::max(p.first.chunks, p.last.chunks);
-  if (blocks + C > 0x7fffffffll) return SFM_ERR_TOO_LARGE;  // (with those that sum the parameters' gradients)
-  first = (unsigned)(B * p.slabs * p.first.chunks);
-  last = (unsigned)(B * p.slabs * p.last.chunks);
+  if (blocks + C > 0x7fffffffll || p.slabs > 65535) return SFM_ERR_TOO_LARGE;  // (with those that sum the parameters' gradients)
+  first = dim3((unsigned)B, p.first.chunks, p.slabs);
+  last = dim3((unsigned)B, p.last.chunks, p.slabs);
   return SFM_OK;
 }
 

@@ -32,8 +32,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
                                                              float2* __restrict__ per_channel) {
   constexpr int A = V / E;
   __shared__ float2 red[kBlock * V];
-  const Where w = where(p, p.first.chunks, blockIdx.x);
-  const Lane l(p, w);
+  const Where w = where(p, blockIdx.x, blockIdx.y, blockIdx.z);
+  const Lane l(p, w, p.row_lanes);
   if (l.mine) {
     const Stream<DT, V> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l);
     Tile t(p, w.chunk);
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
     float mu[A], is[A], ga[V], be[V], s1[V], s2[V];
 #pragma unroll
     for (int a = 0; a < A; ++a) {
-      const long long g = (long long)w.b * p.G + (c + a * E) / p.cpg;
+      const long long g = (long long)w.b * p.G + w.g0 + group_in_slab(p, l.vx * V + a * E);
       mu[a] = mean[g]; is[a] = rstd[g];
     }
 #pragma unroll
@@ -142,8 +142,9 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
     if (lane == 0) { gbeta[c] = (float)a; ggamma[c] = (float)b; }
     return;
   }
-  const Where w = where(p, p.last.chunks, blockIdx.x - param_blocks);
-  const Lane l(p, w);
+  const unsigned bid = blockIdx.x - param_blocks, rest = bid / (unsigned)B;  // (items, chunks, slabs) in one dimension
+  const Where w = where(p, bid - rest * B, rest % (unsigned)p.last.chunks, rest / (unsigned)p.last.chunks);
+  const Lane l(p, w, p.row_lanes);
   const Stream<DT, V, FAR> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l), os(gx, p.C, p, w, l);
   Tile t(p, FAR ? w.chunk : last_tile(p, w));
   Raw<DT, V> xr[kU], gr[kU];
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
     gs.load(t, l.ry, gr);
 #pragma unroll
     for (int a = 0; a < A; ++a) {
-      const long long g = (long long)w.b * p.G + (c + a * E) / p.cpg;
+      const long long g = (long long)w.b * p.G + w.g0 + group_in_slab(p, l.vx * V + a * E);
       mu[a] = mean[g]; is[a] = rstd[g];
     }
 #pragma unroll
@@ -162,21 +163,21 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
   }
   {
     const Team tm = team_of(w.ng);
-    const double inv = 1.0 / ((double)p.N * p.cpg);
+    const float inv = 1.0f / ((float)p.N * (float)p.cpg);
     for (int j = tm.id; j < w.ng; j += tm.count) {
       const float2* src = per_group + ((long long)w.b * p.G + w.g0 + j) * p.P;
-      double a = 0.0, b = 0.0;
+      float a = 0.0f, b = 0.0f;
       for (int q = tm.lane; q < p.P; q += tm.T) { const float2 v = src[q]; a += v.x; b += v.y; }
       a = team_sum(a, tm.T);
       b = team_sum(b, tm.T);
-      if (tm.lane == 0) stat[j] = make_float2((float)(a * inv), (float)(b * inv));
+      if (tm.lane == 0) stat[j] = make_float2(a * inv, b * inv);
     }
     __syncthreads();
   }
   if (!l.mine) return;
 #pragma unroll
   for (int a = 0; a < A; ++a) {
-    const float2 st = stat[(c + a * E) / p.cpg - w.g0];
+    const float2 st = stat[group_in_slab(p, l.vx * V + a * E)];
     c1[a] = st.x;
     c2[a] = st.y;
   }
@@ -228,7 +229,7 @@ extern "C" int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, 
                                       int per_channel, void* gx, float* ggamma, float* gbeta, float* ws, void* stream_) {
   GnPlan p;
   Drop d;
-  unsigned first, last;
+  dim3 first, last;
   const int es = dtype == kF32 ? 4 : 2;
   if (!gy || !ld_gy || n_gy < 1 || n_gy > 3) return SFM_ERR_ARG;
   long long ld = ld_x;
@@ -252,13 +253,13 @@ extern "C" int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, 
   float2* per_channel_sums = per_group + B * G * p.P;
   // a multiple of eight: the workgroups behind them stay on the XCDs they were on in the first launch
   const unsigned params = ggamma ? ((unsigned)(C + kBlock / 64 - 1) / (kBlock / 64) + 7u) / 8u * 8u : 0u;
-  const unsigned second = params + (gx ? last : 0u);
+  const unsigned second = params + (gx ? last.x * last.y * last.z : 0u);
   by_type(dtype, p, [&](auto dt, auto v, auto e) {
     constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
     constexpr int E = decltype(e)::value;
     by_use<DT, V>(threshold != 0, far(3 * B * N * C * es), [&](auto drop, auto away) {
       constexpr bool DROP = decltype(drop)::value;
-      hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, E, DROP>), dim3(first), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta, save_mean,
+      hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, E, DROP>), first, dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta, save_mean,
                          save_rstd, p, (int)B, act, d, per_group, per_channel_sums);
       hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, E, DROP, decltype(away)::value>), dim3(second), dim3(kBlock), 0, stream, x, ld_x, src, gamma, beta,
                          save_mean, save_rstd, p, (int)B, act, d, per_group, per_channel_sums, params, gx, ggamma, gbeta);

@@ -11,18 +11,19 @@ template <int T, int A, int E, typename F>
 __device__ __forceinline__ void reduce_stats(const float2* red, int lanes, int row_lanes, int per_lane, int more, int cg, int ng, F&& out) {
   const Team tm = team_of<T>(ng);
   const int per_row = cg / E, busy = per_lane > 0 ? row_lanes : more;
+  const float per_row_inv = __builtin_amdgcn_rcpf((float)per_row);
   const float rows = (float)per_lane, inv = 1.0f / ((rows * row_lanes + more) * per_row);
   for (int j = tm.id; j < ng; j += tm.count) {
     const float ref = red[j * per_row].x;
     float s = 0.0f;
     for (int e = tm.lane; e < busy * per_row; e += tm.T) {
-      const int row = e / per_row, c = e - row * per_row;
+      const int row = (int)(((float)e + 0.5f) * per_row_inv), c = e - row * per_row;  // e / per_row: e < 2^13, 0.5 / per_row covers the rounding
       s = __builtin_fmaf(rows + (row < more), red[row * lanes * A + j * per_row + c].x - ref, s);
     }
     const float off = team_sum(s, tm.T) * inv;
     float q = 0.0f;
     for (int e = tm.lane; e < busy * per_row; e += tm.T) {
-      const int row = e / per_row, c = e - row * per_row;
+      const int row = (int)(((float)e + 0.5f) * per_row_inv), c = e - row * per_row;  // e / per_row: e < 2^13, 0.5 / per_row covers the rounding
       const float2 v = red[row * lanes * A + j * per_row + c];
       const float d = (v.x - ref) - off;
       q += __builtin_fmaf(E * (rows + (row < more)) * d, d, v.y);
@@ -38,8 +39,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats
                                                           float2* __restrict__ part) {
   constexpr int A = V / E;                   // accumulators
   __shared__ float2 red[kBlock * A];         // [row lane][E channels of the slab]
-  const Where w = where(p, p.first.chunks, blockIdx.x);
-  const Lane l(p, w);
+  const Where w = where(p, blockIdx.x, blockIdx.y, blockIdx.z);
+  const Lane l(p, w, p.row_lanes);
   if (l.mine) {
     const Stream<DT, V> xs(x, ldx, p, w, l);
     float n = 0.0f, mean[A], m2[A];
@@ -99,25 +100,28 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats
   });
 }
 
-// joins the partials of a workgroup's groups: stat[j] = (mean, r) in LDS.  All threads call it; it ends with a barrier.
+__device__ __forceinline__ float rsqrt_of(float var, float eps) { return 1.0f / sqrtf(var + eps); }
+
+// joins the partials of a workgroup's groups: stat[j] = (mean, r) in LDS.  All threads call it; it ends with a barrier.  In fp32: a
+// lane adds few partials, and their means are taken against one of them.
 __device__ __forceinline__ void join_stats(const float2* __restrict__ part, const GnPlan& p, const Where& w, float eps,
                                            float2* __restrict__ stat) {
   const Team t = team_of(w.ng);
-  const double inv = 1.0 / ((double)p.N * p.cpg);
+  const float inv = 1.0f / ((float)p.N * (float)p.cpg);
   for (int j = t.id; j < w.ng; j += t.count) {
     const float2* src = part + ((long long)w.b * p.G + w.g0 + j) * p.P;
     const float ref = src[0].x;
-    double s = 0.0;
-    for (int q = t.lane; q < p.P; q += t.T) s += part_count(p, q) * (src[q].x - ref);
-    const double off = team_sum(s, t.T) * inv;
-    double q2 = 0.0;
+    float s = 0.0f;
+    for (int q = t.lane; q < p.P; q += t.T) s = __builtin_fmaf(part_count(p, q), src[q].x - ref, s);
+    const float off = team_sum(s, t.T) * inv;
+    float q2 = 0.0f;
     for (int q = t.lane; q < p.P; q += t.T) {
       const float2 v = src[q];
-      const double d = (v.x - ref) - off;
-      q2 += v.y + part_count(p, q) * d * d;
+      const float d = (v.x - ref) - off;
+      q2 += __builtin_fmaf(part_count(p, q) * d, d, v.y);
     }
     q2 = team_sum(q2, t.T);
-    if (t.lane == 0) stat[j] = make_float2((float)(ref + off), (float)(1.0 / sqrt(q2 * inv + (double)eps)));
+    if (t.lane == 0) stat[j] = make_float2(ref + off, rsqrt_of(q2 * inv, eps));
   }
   __syncthreads();
 }
@@ -132,8 +136,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
                                                           float* __restrict__ save_r) {
   constexpr int A = V / E;
   __shared__ float2 stat[kBlock * A];
-  const Where w = where(p, p.last.chunks, blockIdx.x);
-  const Lane l(p, w);
+  const Where w = where(p, blockIdx.x, blockIdx.y, blockIdx.z);
+  const Lane l(p, w, p.row_lanes);
   const Stream<DT, V, FAR> xs(x, ldx, p, w, l), ys(y, ldy, p, w, l);
   Tile t(p, FAR ? w.chunk : last_tile(p, w));
   Raw<DT, V> raw[kU];
@@ -154,7 +158,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
   float mu[A];
 #pragma unroll
   for (int a = 0; a < A; ++a) {
-    const float2 st = stat[(c + a * E) / p.cpg - w.g0];
+    const float2 st = stat[group_in_slab(p, l.vx * V + a * E)];
     mu[a] = st.x;
 #pragma unroll
     for (int k = a * E; k < (a + 1) * E; ++k) sc[k] *= st.y;
@@ -202,20 +206,19 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
                                                     float* __restrict__ save_r) {
   constexpr int A = V / E, kES = ElemBytes<DT>::value;
   __shared__ float2 red[T * A], stat[T * A];
-  const Where w = where(p, 1, blockIdx.x);
+  const Where w = where(p, blockIdx.x, 0, blockIdx.y);
   const int N = (int)p.N, row_lanes = T / p.lanes;
-  const int vx = threadIdx.x % (unsigned)p.lanes, ry = threadIdx.x / (unsigned)p.lanes;
-  const bool mine = ry < row_lanes && vx * V < w.cc;
+  const Lane l(p, w, row_lanes);
   const int per_lane = N / row_lanes, more = N % row_lanes;
-  const int rows = mine ? per_lane + (ry < more) : 0;  // of this thread
-  const int c = w.c0 + vx * V;
-  const char* xs = static_cast<const char*>(x) + ((long long)w.b * N * ldx + c) * kES + ry * ldx * kES;
+  const int rows = l.mine ? per_lane + (l.ry < more) : 0;  // of this thread
+  const int c = w.c0 + l.vx * V;
+  const char* xs = static_cast<const char*>(x) + ((long long)w.b * N * ldx + c) * kES + l.ry * ldx * kES;
   Raw<DT, V> raw[kHeld];
 #pragma unroll
   for (int u = 0; u < kHeld; ++u)
     if (u < rows) raw[u] = load_raw<DT, V>(xs, (long long)u * row_lanes * ldx * kES);
   float sc[V], sh[V];
-  if (mine) {
+  if (l.mine) {
 #pragma unroll
     for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k]; sh[k] = beta[c + k]; }
     float s[A], q[A];
@@ -241,12 +244,12 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
         for (int k = 0; k < V; ++k) { const float d = f[k] - s[k / E]; q[k / E] = __builtin_fmaf(d, d, q[k / E]); }
       }
 #pragma unroll
-    for (int a = 0; a < A; ++a) red[(ry * p.lanes + vx) * A + a] = make_float2(s[a], q[a]);
+    for (int a = 0; a < A; ++a) red[(l.ry * p.lanes + l.vx) * A + a] = make_float2(s[a], q[a]);
   }
   __syncthreads();
   const float inv = 1.0f / ((float)N * (float)p.cpg);
   reduce_stats<T, A, E>(red, p.lanes, row_lanes, per_lane, more, p.cpg, w.ng, [&](int j, float mean, float m2) {
-    const float r = 1.0f / sqrtf(__builtin_fmaf(m2, inv, eps));
+    const float r = rsqrt_of(m2 * inv, eps);
     stat[j] = make_float2(mean, r);
     if (save_mean) {
       save_mean[(long long)w.b * p.G + w.g0 + j] = mean;
@@ -254,11 +257,11 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
     }
   });
   __syncthreads();
-  if (!mine) return;
+  if (!l.mine) return;
   float mu[A];
 #pragma unroll
   for (int a = 0; a < A; ++a) {
-    const float2 st = stat[(c + a * E) / p.cpg - w.g0];
+    const float2 st = stat[group_in_slab(p, l.vx * V + a * E)];
     mu[a] = st.x;
 #pragma unroll
     for (int k = a * E; k < (a + 1) * E; ++k) sc[k] *= st.y;
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
     key = drop_key(drop);
     if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
   }
-  char* ys = static_cast<char*>(y) + ((long long)w.b * N * ldy + c) * kES + ry * ldy * kES;
+  char* ys = static_cast<char*>(y) + ((long long)w.b * N * ldy + c) * kES + l.ry * ldy * kES;
 #pragma unroll
   for (int u = 0; u < kHeld; ++u) {
     if (u < rows) {
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
       act_fwd<V>(f, act);
       if (DROP) {
         if (!drop.per_channel)
-          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(u * row_lanes + ry) * p.C + c);
+          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(u * row_lanes + l.ry) * p.C + c);
         drop_apply<V>(f, keep, drop.scale);
       }
       store_vec<DT, V>(ys, (long long)u * row_lanes * ldy * kES, f);
@@ -303,7 +306,7 @@ using namespace sfm;
 
 extern "C" long long sfm_group_norm_workspace_floats(long long B, long long N, int C, int G, int dtype, int backward) {
   GnPlan p;
-  unsigned first, last;
+  dim3 first, last;
   const int rc = gn_setup(B, N, C, G, dtype, C, backward != 0, p, first, last);
   if (rc) return rc;
   return 2 * (B * G * p.P + (backward ? B * C * p.first.chunks : 0));
@@ -315,7 +318,7 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
                                       long long ld_y, float* save_mean, float* save_rstd, float* ws, void* stream_) {
   GnPlan p;
   Drop d;
-  unsigned first, last;
+  dim3 first, last;
   const int es = dtype == kF32 ? 4 : 2;
   const int rc = gn_setup(B, N, C, G, dtype, std::max(ld_x, ld_y), false, p, first, last);
   if (rc) return rc;
@@ -327,14 +330,13 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
   hipStream_t stream = (hipStream_t)stream_;
   float2* part = reinterpret_cast<float2*>(ws);
   const int held = held_threads(p, es);
-  const unsigned slabs = (unsigned)(B * p.slabs);
   by_type(dtype, p, [&](auto dt, auto v, auto e) {
     constexpr int DT = decltype(dt)::value, V = decltype(v)::value;
     constexpr int E = decltype(e)::value;
     if constexpr (V * ElemBytes<DT>::value == 16) {
       auto one = [&](auto threads, auto drop) {
         constexpr int T = decltype(threads)::value;
-        hipLaunchKernelGGL((gn_held_kernel<DT, V, E, decltype(drop)::value, T>), dim3(slabs), dim3(T), 0, stream, x, ld_x, gamma, beta, p,
+        hipLaunchKernelGGL((gn_held_kernel<DT, V, E, decltype(drop)::value, T>), dim3((unsigned)B, p.slabs), dim3(T), 0, stream, x, ld_x, gamma, beta, p,
                            eps, act, d, y, ld_y, save_mean, save_rstd);
       };
       auto with = [&](auto threads) { threshold ? one(threads, std::true_type{}) : one(threads, std::false_type{}); };
@@ -342,8 +344,8 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
       if (held == 1024) return with(std::integral_constant<int, 1024>{});
     }
     by_use<DT, V>(threshold != 0, far(2 * B * N * C * es), [&](auto drop, auto away) {
-      hipLaunchKernelGGL((gn_stats_kernel<DT, V, E>), dim3(first), dim3(kBlock), 0, stream, x, ld_x, p, part);
-      hipLaunchKernelGGL((gn_apply_kernel<DT, V, E, decltype(drop)::value, decltype(away)::value>), dim3(last), dim3(kBlock), 0, stream,
+      hipLaunchKernelGGL((gn_stats_kernel<DT, V, E>), first, dim3(kBlock), 0, stream, x, ld_x, p, part);
+      hipLaunchKernelGGL((gn_apply_kernel<DT, V, E, decltype(drop)::value, decltype(away)::value>), last, dim3(kBlock), 0, stream,
                          x, ld_x, gamma, beta, part, p, eps, act, d, y, ld_y, save_mean, save_rstd);
     });
   });
