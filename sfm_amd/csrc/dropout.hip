@@ -9,12 +9,12 @@ constexpr int kPer = 4;  // blocks of eight elements a thread draws for; a workg
 
 // the eight keep bits of block `blk` of an item
 __device__ __forceinline__ unsigned keep_eight(const Drop& d, const DropKey& key, unsigned item, unsigned blk, unsigned C) {
-  if (!d.per_channel) return keep_bits<8>(d, key, d.item0 + item, (unsigned long long)blk * 8);
-  if (C % 8 == 0) return keep_bits<8>(d, key, d.item0 + item, blk % (C / 8) * 8);
+  if (!d.per_channel) return keep_bits(d, key, d.item0 + item, (unsigned long long)blk * 8);
+  if (C % 8 == 0) return keep_bits(d, key, d.item0 + item, blk % (C / 8) * 8);
   unsigned keep = 0, c = (unsigned)((unsigned long long)blk * 8 % C), have = ~0u, eight = 0;  // they cross from row to row
 #pragma unroll 1
   for (int e = 0; e < 8; ++e) {
-    if ((c >> 3) != have) { have = c >> 3; eight = keep_bits<8>(d, key, d.item0 + item, c & ~7u); }
+    if ((c >> 3) != have) { have = c >> 3; eight = keep_bits(d, key, d.item0 + item, c & ~7u); }
     keep |= ((eight >> (c & 7)) & 1u) << e;
     c = c + 1 == C ? 0 : c + 1;
   }
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kBlock) void dropout_blocks_kernel(const char* __re
       if (first + lane / R >= left) continue;
       float f[V];
       unpack<DT, V>(raw[k][r], f);
-      drop_apply<V>(f, bits, d.scale);
+      keep_apply<V>(f, bits, d.scale);
       store_vec<DT, V, FAR>(ys, (first * 8 + lane * V) * (unsigned)ElemBytes<DT>::value, f);
     }
   }
@@ -82,13 +82,13 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const char* __restrict_
     if (first + 8 <= n) {
       float f[8];
       unpack<DT, 8>(load_raw<DT, 8>(x, at), f);
-      drop_apply<8>(f, keep, d.scale);
+      keep_apply<8>(f, keep, d.scale);
       store_vec<DT, 8>(y, at, f);
     } else {
       for (unsigned e = 0; first + e < n; ++e) {
         float f[1];
         unpack<DT, 1>(load_raw<DT, 1>(x, at + e * kBytes), f);
-        drop_apply<1>(f, keep >> e, d.scale);
+        keep_apply<1>(f, keep >> e, d.scale);
         store_vec<DT, 1>(y, at + e * kBytes, f);
       }
     }

@@ -60,6 +60,7 @@ struct GnPlan {
     int extra;
     int owner;           // the chunk of the last tile
   } first, last;         // the pass that makes partial sums, and the one that joins and applies them
+  bool pairs;            // lanes 2i and 2i + 1 always hold the halves of a block of eight channels (fp32; draw_pair)
   int P;                 // partials of a group: first.chunks * parts
 };
 
@@ -114,6 +115,7 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, bool backwar
     p.slabs = G * p.parts;
   }
   p.lanes = p.cs / p.V;
+  p.pairs = p.V == 4 && es == 4 && C % 8 == 0 && p.cs % 8 == 0;
   p.lanes_inv = ((1u << 20) + p.lanes - 1) / p.lanes;
   p.cpg_inv = p.cpg == 1 ? 0u : (unsigned)(((1ull << 32) + p.cpg - 1) / p.cpg);
   gn_tiles(p, kBlock / p.lanes);
@@ -218,6 +220,34 @@ template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, f
   __device__ __forceinline__ void store(const char* a, int u, const float (&f)[V]) const {
     store_vec<DT, V, NT>(const_cast<char*>(a) + u * step, off, f);
   }
+};
+
+// The mask of a thread's vector in the rows of a tile, u ascending from 0 in every tile.
+template <int V> struct Mask {
+  const Drop& d;
+  DropKey key;
+  unsigned item;
+  bool pairs;
+  Draw<V> now, next;
+  __device__ __forceinline__ Mask(const Drop& drop, const GnPlan& p, const Where& w, int channel)
+      : d(drop), key(drop_key(drop)), item(drop.item0 + w.b), pairs(p.pairs) {
+    if (d.per_channel) now = draw<V>(d, key, item, channel);
+  }
+  // place: of the vector in row u; step: places between rows u and u + 1
+  __device__ __forceinline__ void apply(float (&f)[V], int u, unsigned long long place, unsigned long long step) {
+    if (!d.per_channel) {
+      if constexpr (V == 4) {
+        if (pairs) {
+          if (u & 1) now = next;
+          else draw_pair(d, key, item, place, step, now, next);
+        } else now = draw<V>(d, key, item, place);
+      } else now = draw<V>(d, key, item, place);
+    }
+    drop_apply<V>(f, now, d);
+  }
+};
+struct NoMask {
+  template <typename... T> __device__ __forceinline__ NoMask(const T&...) {}
 };
 
 // Teams: the workgroup's threads, cut into teams of T lanes of one wave (T a power of two), one group each at a time.

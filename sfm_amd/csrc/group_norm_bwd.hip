@@ -49,13 +49,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) { ga[k] = gamma[c + k]; be[k] = beta[c + k]; s1[k] = 0.0f; s2[k] = 0.0f; }
-    DropKey key{};
-    unsigned keep = 0;
-    if (DROP) {
-      key = drop_key(drop);
-      if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
-    }
-    const unsigned long long place = (unsigned long long)l.ry * p.C + c;
+  std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
+    const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
     for (;;) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
@@ -64,11 +59,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
         unpack<DT, V>(xr[u], f);
         unpack<DT, V>(gr[u], g);
         if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, l, t, u, g);
-        if (DROP) {
-          if (!drop.per_channel)
-            keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
-          drop_apply<V>(g, keep, drop.scale);
-        }
+        if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * kU + u) * row_places + place, row_places);
 #pragma unroll
         for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
         act_bwd<V>(g, z, act);
@@ -181,13 +172,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
     c1[a] = st.x;
     c2[a] = st.y;
   }
-  DropKey key{};
-  unsigned keep = 0;
-  if (DROP) {
-    key = drop_key(drop);
-    if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
-  }
-  const unsigned long long place = (unsigned long long)l.ry * p.C + c;
+  std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
+  const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
   for (;;) {
     const char* o = os.at(t);
 #pragma unroll
@@ -197,11 +183,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
       unpack<DT, V>(xr[u], f);
       unpack<DT, V>(gr[u], g);
       if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, l, t, u, g);
-      if (DROP) {
-        if (!drop.per_channel)
-          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
-        drop_apply<V>(g, keep, drop.scale);
-      }
+      if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * kU + u) * row_places + place, row_places);
 #pragma unroll
       for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
       act_bwd<V>(g, z, act);

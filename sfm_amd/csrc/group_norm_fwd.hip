@@ -163,13 +163,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
 #pragma unroll
     for (int k = a * E; k < (a + 1) * E; ++k) sc[k] *= st.y;
   }
-  DropKey key{};
-  unsigned keep = 0;
-  if (DROP) {
-    key = drop_key(drop);
-    if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
-  }
-  const unsigned long long place = (unsigned long long)l.ry * p.C + c;
+  std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
+  const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
   for (;;) {
     const bool more = FAR ? t.index + p.last.chunks < p.tiles : t.index >= p.last.chunks;
     const Tile next(p, !more ? t.index : FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
@@ -183,11 +178,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
       act_fwd<V>(f, act);
-      if (DROP) {
-        if (!drop.per_channel)
-          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(t.index * kU + u) * p.row_lanes * p.C + place);
-        drop_apply<V>(f, keep, drop.scale);
-      }
+      if constexpr (DROP) mask.apply(f, u, (unsigned long long)(t.index * kU + u) * row_places + place, row_places);
       if (t.valid(u, l.ry)) ys.store(o, u, f);
     }
     if (!more) break;
@@ -266,12 +257,7 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
 #pragma unroll
     for (int k = a * E; k < (a + 1) * E; ++k) sc[k] *= st.y;
   }
-  DropKey key{};
-  unsigned keep = 0;
-  if (DROP) {
-    key = drop_key(drop);
-    if (drop.per_channel) keep = keep_bits<V>(drop, key, drop.item0 + w.b, c);
-  }
+  std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
   char* ys = static_cast<char*>(y) + ((long long)w.b * N * ldy + c) * kES + l.ry * ldy * kES;
 #pragma unroll
   for (int u = 0; u < kHeld; ++u) {
@@ -281,11 +267,7 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
       act_fwd<V>(f, act);
-      if (DROP) {
-        if (!drop.per_channel)
-          keep = keep_bits<V>(drop, key, drop.item0 + w.b, (unsigned long long)(u * row_lanes + l.ry) * p.C + c);
-        drop_apply<V>(f, keep, drop.scale);
-      }
+      if constexpr (DROP) mask.apply(f, u, (unsigned long long)(u * row_lanes + l.ry) * p.C + c, (unsigned long long)row_lanes * p.C);
       store_vec<DT, V>(ys, (long long)u * row_lanes * ldy * kES, f);
     }
   }

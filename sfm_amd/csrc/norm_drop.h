@@ -110,17 +110,9 @@ constexpr float kLog2e = 1.44269504088896341f;
 // Results under 2^-126 become 0, which no activation below can tell from what they are.
 __device__ __forceinline__ float exp_fast(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 
-// e^z - 1 for z <= 0.  e^z - 1 itself loses everything for small |z| (an absolute 2^-24 on a result of size |z|), so above -0.35
-// it is the Taylor polynomial to z^7 / 7! (what is left out is under 0.35^7 / 8! = 1.6e-8 of the result).
-__device__ __forceinline__ float expm1_neg(float z) {
-  float p = __builtin_fmaf(z, 1.0f / 5040.0f, 1.0f / 720.0f);
-  p = __builtin_fmaf(p, z, 1.0f / 120.0f);
-  p = __builtin_fmaf(p, z, 1.0f / 24.0f);
-  p = __builtin_fmaf(p, z, 1.0f / 6.0f);
-  p = __builtin_fmaf(p, z, 0.5f);
-  p = __builtin_fmaf(p * z, z, z);
-  return z > -0.35f ? p : exp_fast(z) - 1.0f;
-}
+// e^z - 1 as it stands: an absolute 2^-24 for small |z|, where z itself, a sum of terms of size 1, is no more exact.  (A polynomial
+// below 0.35 made it relative and cost 9 of 20 operations an element: 13.6 MB of bf16 activations 14.2 us, 12.3 without.)
+__device__ __forceinline__ float elu(float z) { return z > 0.0f ? z : exp_fast(z) - 1.0f; }
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_fast(-z)); }
 
@@ -128,7 +120,7 @@ template <int V>
 __device__ __forceinline__ void act_fwd(float (&z)[V], int act) {  // act is uniform
   if (act == kActElu) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) z[k] = z[k] > 0.0f ? z[k] : expm1_neg(z[k]);
+    for (int k = 0; k < V; ++k) z[k] = elu(z[k]);
   } else if (act == kActRelu) {
 #pragma unroll
     for (int k = 0; k < V; ++k) z[k] = z[k] < 0.0f ? 0.0f : z[k];  // a NaN stays one
@@ -191,22 +183,64 @@ __device__ __forceinline__ uint4 philox7(unsigned c0, unsigned c1, unsigned c2, 
   return make_uint4(c0, c1, c2, c3);
 }
 
-// keep bits of elements place .. place + V - 1 of an item, bit k for element k.  V is a power of two <= 8 that divides place: the
-// V elements lie in one block of eight.
+__device__ __forceinline__ uint4 block_words(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
+  return philox7((unsigned)(place >> 3), item, key.step, d.layer, key.k0, key.k1);
+}
+
+// the 16-bit numbers of elements place .. place + V - 1 of an item, two in a word.  V is a power of two <= 8 that divides place: the V
+// elements lie in one block of eight.
+template <int V> struct Draw { unsigned w[(V + 1) / 2]; };
 template <int V>
-__device__ __forceinline__ unsigned keep_bits(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
-  const uint4 r = philox7((unsigned)(place >> 3), item, key.step, d.layer, key.k0, key.k1);
-  const unsigned w[4] = {r.x, r.y, r.z, r.w};
-  unsigned all = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) all |= ((k & 1 ? w[k / 2] >> 16 : w[k / 2] & 0xffffu) >= d.threshold ? 1u : 0u) << k;
-  return V == 8 ? all : all >> (unsigned)(place & 7);
+__device__ __forceinline__ Draw<V> draw(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
+  const uint4 r = block_words(d, key, item, place);
+  Draw<V> o;
+  if constexpr (V == 8) { o.w[0] = r.x; o.w[1] = r.y; o.w[2] = r.z; o.w[3] = r.w; }
+  else if constexpr (V == 4) { o.w[0] = place & 4 ? r.z : r.x; o.w[1] = place & 4 ? r.w : r.y; }
+  else {
+    const unsigned lo = place & 2 ? r.y : r.x, hi = place & 2 ? r.w : r.z, w = place & 4 ? hi : lo;
+    o.w[0] = V == 2 || !(place & 1) ? w : w >> 16;
+  }
+  return o;
+}
+
+// Two draws of four elements by lanes 2i and 2i + 1 that hold the two halves of one block of eight in each of two rows: the even lane
+// draws the first row's block, the odd one the second's, and they swap the halves (a quad permutation): one draw a lane for
+// eight elements, not two.
+__device__ __forceinline__ void draw_pair(const Drop& d, const DropKey& key, unsigned item, unsigned long long place,
+                                          unsigned long long row, Draw<4>& first, Draw<4>& second) {
+  const bool odd = threadIdx.x & 1;
+  const uint4 r = block_words(d, key, item, place + (odd ? row : 0));
+  const unsigned s0 = odd ? r.x : r.z, s1 = odd ? r.y : r.w;  // what the other lane needs
+  const unsigned o0 = __builtin_amdgcn_update_dpp(0, (int)s0, 0xB1, 0xF, 0xF, true);
+  const unsigned o1 = __builtin_amdgcn_update_dpp(0, (int)s1, 0xB1, 0xF, 0xF, true);
+  first.w[0] = odd ? o0 : r.x;
+  first.w[1] = odd ? o1 : r.y;
+  second.w[0] = odd ? r.z : o0;
+  second.w[1] = odd ? r.w : o1;
 }
 
 template <int V>
-__device__ __forceinline__ void drop_apply(float (&f)[V], unsigned keep, float scale) {
+__device__ __forceinline__ void drop_apply(float (&f)[V], const Draw<V>& r, const Drop& d) {
+  const unsigned t = d.threshold << 16;
 #pragma unroll
-  for (int k = 0; k < V; ++k) f[k] = (keep >> k) & 1 ? f[k] * scale : 0.0f;  // a dropped infinity or NaN is 0 as well
+  for (int k = 0; k < V; ++k)  // a dropped infinity or NaN is 0 as well
+    f[k] = (k & 1 ? r.w[k / 2] : r.w[k / 2] << 16) >= t ? f[k] * d.scale : 0.0f;
+}
+
+// the same as bits: what a lane hands to others
+__device__ __forceinline__ unsigned keep_bits(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
+  const uint4 r = block_words(d, key, item, place);
+  const unsigned w[4] = {r.x, r.y, r.z, r.w}, t = d.threshold << 16;
+  unsigned all = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) all |= ((k & 1 ? w[k / 2] : w[k / 2] << 16) >= t ? 1u : 0u) << k;
+  return all;
+}
+
+template <int V>
+__device__ __forceinline__ void keep_apply(float (&f)[V], unsigned keep, float scale) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) f[k] = (keep >> k) & 1 ? f[k] * scale : 0.0f;
 }
 
 // the arguments of one mask as the C ABI passes them -> false if they are none
