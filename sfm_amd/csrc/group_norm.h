@@ -59,6 +59,7 @@ struct GnPlan {
     long long own;       // tiles of a chunk; the first `extra` chunks have one more
     int extra;
     int owner;           // the chunk of the last tile
+    float rows, rows_more;  // rows of a chunk of `own` tiles and of one more, were the last tile full
   } first, last;         // the pass that makes partial sums, and the one that joins and applies them
   bool pairs;            // lanes 2i and 2i + 1 always hold the halves of a block of eight channels (fp32; draw_pair)
   int P;                 // partials of a group: first.chunks * parts
@@ -80,6 +81,8 @@ static void gn_tiles(GnPlan& p, int row_lanes) {
     t->own = p.tiles / t->chunks;
     t->extra = (int)(p.tiles % t->chunks);
     t->owner = (int)((p.tiles - 1) % t->chunks);
+    t->rows = (float)(t->own * p.tile_rows);
+    t->rows_more = (float)((t->own + 1) * p.tile_rows);
   }
 }
 
@@ -262,11 +265,24 @@ template <typename F> __device__ __forceinline__ F team_sum(F v, int T) {
   return v;
 }
 
+// f(k, value) for k = first, first + step, ... < n of src, K loads on their way at a time: partial sums have been written by
+// workgroups all over the chip, a load of one takes about a microsecond, and one after the other they were most of a small pass
+template <int K, typename F> __device__ __forceinline__ void each_partial(const float2* __restrict__ src, long long n, int first, int step, F&& f) {
+  for (long long base = first; base < n; base += K * step) {
+    float2 v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = src[min(base + k * step, n - 1)];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (base + k * step < n) f((int)(base + k * step), v[k]);
+  }
+}
+
 // values that partial q of a group covers
 __device__ __forceinline__ float part_count(const GnPlan& p, int q) {
   const int chunk = p.parts == 1 ? q : q / p.parts, part = q - chunk * p.parts;
-  const long long rows = (p.first.own + (chunk < p.first.extra)) * p.tile_rows - (chunk == p.first.owner ? p.tile_rows - p.left : 0);
-  return (float)rows * (float)(p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
+  const float rows = (chunk < p.first.extra ? p.first.rows_more : p.first.rows) - (chunk == p.first.owner ? (float)(p.tile_rows - p.left) : 0.0f);
+  return rows * (float)(p.parts == 1 ? p.cpg : min(p.cs, p.cpg - part * p.cs));
 }
 
 // dispatch on the type, the vector width, and how many adjacent channels of a vector are of one group (a power of two that divides

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
     const long long n = (long long)B * p.first.chunks;
     const float2* src = per_channel + c * n;
     double a = 0.0, b = 0.0;
-    for (long long k = lane; k < n; k += 64) { const float2 v = src[k]; a += v.x; b += v.y; }
+    each_partial<8>(src, n, lane, 64, [&](int, float2 v) { a += v.x; b += v.y; });
     a = team_sum(a, 64);
     b = team_sum(b, 64);
     if (lane == 0) { gbeta[c] = (float)a; ggamma[c] = (float)b; }
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
     for (int j = tm.id; j < w.ng; j += tm.count) {
       const float2* src = per_group + ((long long)w.b * p.G + w.g0 + j) * p.P;
       float a = 0.0f, b = 0.0f;
-      for (int q = tm.lane; q < p.P; q += tm.T) { const float2 v = src[q]; a += v.x; b += v.y; }
+      each_partial<4>(src, p.P, tm.lane, tm.T, [&](int, float2 v) { a += v.x; b += v.y; });
       a = team_sum(a, tm.T);
       b = team_sum(b, tm.T);
       if (tm.lane == 0) stat[j] = make_float2(a * inv, b * inv);

@@ -102,23 +102,49 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats
 
 __device__ __forceinline__ float rsqrt_of(float var, float eps) { return 1.0f / sqrtf(var + eps); }
 
-// joins the partials of a workgroup's groups: stat[j] = (mean, r) in LDS.  All threads call it; it ends with a barrier.  In fp32: a
-// lane adds few partials, and their means are taken against one of them.
-__device__ __forceinline__ void join_stats(const float2* __restrict__ part, const GnPlan& p, const Where& w, float eps,
+// joins the partials of a workgroup's groups: stat[j] = (mean, r) in LDS.  All threads call it; it ends with a barrier.  In fp32, a
+// lane adds few of them, and with the means taken against one of them; fp64 in one pass over them took 1.2 us more of a small pass.
+// K: loads on their way at a time, what the registers allow beside the batch of x that is on its way as well.
+template <int K> __device__ __forceinline__ void join_stats(const float2* __restrict__ part, const GnPlan& p, const Where& w, float eps,
                                            float2* __restrict__ stat) {
   const Team t = team_of(w.ng);
   const float inv = 1.0f / ((float)p.N * (float)p.cpg);
   for (int j = t.id; j < w.ng; j += t.count) {
     const float2* src = part + ((long long)w.b * p.G + w.g0 + j) * p.P;
     const float ref = src[0].x;
-    float s = 0.0f;
-    for (int q = t.lane; q < p.P; q += t.T) s = __builtin_fmaf(part_count(p, q), src[q].x - ref, s);
-    const float off = team_sum(s, t.T) * inv;
-    float q2 = 0.0f;
-    for (int q = t.lane; q < p.P; q += t.T) {
-      const float2 v = src[q];
-      const float d = (v.x - ref) - off;
-      q2 += __builtin_fmaf(part_count(p, q) * d, d, v.y);
+    float s = 0.0f, q2 = 0.0f, off;
+    if (p.parts == 1) {
+      const float more = p.first.rows_more * p.cpg, rows = p.first.rows * p.cpg, less = (float)(p.tile_rows - p.left) * p.cpg;
+      auto count = [&](int q) { return (q < p.first.extra ? more : rows) - (q == p.first.owner ? less : 0.0f); };
+      float2 v[K];  // the first K of the lane are loaded once
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = src[min(t.lane + k * t.T, p.P - 1)];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int q = t.lane + k * t.T;
+        v[k].x -= ref;
+        if (q < p.P) s = __builtin_fmaf(count(q), v[k].x, s);
+      }
+      each_partial<K>(src, p.P, t.lane + K * t.T, t.T, [&](int q, float2 u) { s = __builtin_fmaf(count(q), u.x - ref, s); });
+      off = team_sum(s, t.T) * inv;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int q = t.lane + k * t.T;
+        const float d = v[k].x - off;
+        if (q < p.P) q2 += __builtin_fmaf(count(q) * d, d, v[k].y);
+      }
+      each_partial<K>(src, p.P, t.lane + K * t.T, t.T, [&](int q, float2 u) {
+        const float d = (u.x - ref) - off;
+        q2 += __builtin_fmaf(count(q) * d, d, u.y);
+      });
+    } else {
+      for (int q = t.lane; q < p.P; q += t.T) s = __builtin_fmaf(part_count(p, q), src[q].x - ref, s);
+      off = team_sum(s, t.T) * inv;
+      for (int q = t.lane; q < p.P; q += t.T) {
+        const float2 u = src[q];
+        const float d = (u.x - ref) - off;
+        q2 += __builtin_fmaf(part_count(p, q) * d, d, u.y);
+      }
     }
     q2 = team_sum(q2, t.T);
     if (t.lane == 0) stat[j] = make_float2(ref + off, rsqrt_of(q2 * inv, eps));
@@ -148,7 +174,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
 #pragma unroll
     for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k]; sh[k] = beta[c + k]; }
   }
-  join_stats(part, p, w, eps, stat);
+  join_stats<DT == kF32 ? 2 : 4>(part, p, w, eps, stat);
   if (save_mean && w.chunk == 0 && w.part == 0)
     for (int j = threadIdx.x; j < w.ng; j += kBlock) {
       save_mean[(long long)w.b * p.G + w.g0 + j] = stat[j].x;
