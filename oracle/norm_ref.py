@@ -83,3 +83,61 @@ def group_norm_act(x, gamma, beta, groups, eps, kind, gy=None, keep=None, thresh
                                                             + np.abs(xhat).max(axis=(1, 3), keepdims=True)),
                                     v.shape).reshape(x.shape)
     return out
+
+
+# ---- the decoder with group norm and dropout, in torch float64 on the CPU: ref_graph's wiring with another normaliser
+def _torch_norm(x, q, groups, activation, mask, name_index):
+    import torch
+    B, C = x.shape[0], x.shape[-1]
+    v = x.reshape(B, -1, groups, C // groups)
+    var, mean = torch.var_mean(v, dim=(1, 3), unbiased=False, keepdim=True)
+    z = ((v - mean) / torch.sqrt(var + 1e-5)).reshape(x.shape) * q["gamma"] + q["beta"]
+    if not activation:
+        return z
+    y = torch.where(z > 0, z, torch.expm1(z.clamp(max=0)))
+    if mask is not None and name_index is not None:
+        t = mask["threshold"]
+        keep = keep_mask(tuple(x.shape), t, mask["seed"], mask["step"], mask["layer"] + name_index, mask["per_channel"], mask["first_item"])
+        y = y * torch.from_numpy(keep.astype(np.float64)) * (65536 / (65536 - t))
+    return y
+
+
+def level(params, concat, skip_feat=None, rates=(2, 4), use_skip=True, use_skip2=True, skip2=None, groups=8, mask=None):
+    """sfm_amd.disp_bottleneck_dense(..., groups=groups, dropout=mask); mask: dict(threshold, seed, step, layer, per_channel, first_item)"""
+    import torch
+    from . import ref_graph as R
+    place = {"sup": 0, "aspp_up": 1, "aspp_up2": 2, "skip": 3, "skip2": 4}
+
+    def sc(x, name, rate=None, activation=True):
+        q = params[name]
+        y = R.conv1x1(x, q["w"]) if rate is None else R.dilated_conv3x3(x, q["w"], rate)
+        return _torch_norm(y, q, groups, activation, mask, place.get(name))
+    h, w = concat.shape[1], concat.shape[2]
+    upnet = sc(R.resize_bilinear_tf1(concat, 2 * h, 2 * w), "up", activation=False)
+    sup = sc(upnet, "sup")
+    a1 = sc(upnet, "aspp_up", rate=rates[0])
+    a2 = sc(torch.cat([sup, a1], dim=3), "aspp_up2", rate=rates[1])
+    if use_skip:
+        skip = sc(_torch_norm(skip_feat, params["skip_bn"], groups, True, None, None), "skip")
+    else:
+        skip = sc(torch.cat([a1, a2], dim=3), "skip", rate=rates[1] * 2)
+    parts = [sup, a1, a2, skip]
+    if use_skip2:
+        parts.append(sc(R.resize_bilinear_tf1(skip2, 2 * h, 2 * w), "skip2"))
+    return sc(torch.cat(parts, dim=3), "out", activation=False), upnet
+
+
+def decoder(end_points, params, groups=8, mask=None):
+    """sfm_amd.disp_aspp_u_dense_decoder(..., groups=groups, dropout=mask)"""
+    from . import ref_graph as R
+
+    def lvl(k, name, *a, **kw):
+        return level(params[name], *a, groups=groups, mask=None if mask is None else {**mask, "layer": mask["layer"] + 8 * k}, **kw)
+    x = _torch_norm(end_points["block4"], params["stem_bn"], groups, True, None, None)
+    x = _torch_norm(R.conv1x1(x, params["stem"]["w"]), params["stem"], groups, False, None, None)
+    x, _ = lvl(0, "concat", x, end_points["block3"], use_skip2=False)
+    x, s1 = lvl(1, "concat1", x, end_points["block2"], use_skip2=False)
+    x2, s2 = lvl(2, "concat2", x, end_points["block1"], skip2=s1)
+    x3, s3 = lvl(3, "concat3", x2, end_points["root_block"], rates=(3, 6), skip2=s2)
+    x4, _ = lvl(4, "concat4", x3, None, rates=(3, 6), use_skip=False, skip2=s3)
+    return [R.disp_head(x, params[n]["w"], params[n]["b"]) for x, n in ((x4, "disp4"), (x3, "disp3"), (x2, "disp2"))]

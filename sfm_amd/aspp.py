@@ -10,6 +10,7 @@ resnet/resnet_utils.py:232-251; csrc/bn_elu.hip), and ``conv2d_bn_elu`` chains t
 """
 from __future__ import annotations
 
+import contextlib
 import weakref
 
 import torch
@@ -319,12 +320,34 @@ def conv1x1(x: Tensor, w: Tensor) -> Tensor:
     return _Conv1x1.apply(x, w)
 
 
-def _slim_conv(x, p, name, rate=None, activation=True, process_group=None):
+def _normalise(x, q, activation, process_group, groups, mask):
+    """batch norm (groups None) or group norm, the ELU if asked for, and the mask if there is one"""
+    from . import norm
+    if groups is not None:
+        return norm.group_norm_act(x, q["gamma"], q["beta"], groups, activation="elu" if activation else None, dropout=mask)
+    y = batch_norm_elu(x, q["gamma"], q["beta"], q.get("moving_mean"), q.get("moving_var"), activation=activation,
+                       process_group=process_group)
+    return y if mask is None else norm.dropout(y, mask)
+
+
+def _slim_conv(x, p, name, rate=None, activation=True, process_group=None, groups=None, masks=None):
     """one slim.conv2d of the block under its arg-scope: p[name] = dict(w, gamma, beta[, moving_mean, moving_var])"""
     q = p[name]
     y = conv1x1(x, q["w"]) if rate is None else dilated_conv3x3(x, q["w"], rate)
-    return batch_norm_elu(y, q["gamma"], q["beta"], q.get("moving_mean"), q.get("moving_var"), activation=activation,
-                          process_group=process_group)
+    return _normalise(y, q, activation, process_group, groups, masks.get(name) if masks else None)
+
+
+# the activations of a level that a mask drops from, each with a draw of its own (layer = the mask's plus its place here)
+_LEVEL_DRAWS = ("sup", "aspp_up", "aspp_up2", "skip", "skip2")
+
+
+def _level_masks(dropout):
+    if dropout is None:
+        return {}
+    from .norm import DropoutMask
+    if not isinstance(dropout, DropoutMask):
+        raise TypeError(f"dropout must be a DropoutMask, got {type(dropout).__name__}")
+    return {nm: dropout.for_layer(dropout.layer + k) for k, nm in enumerate(_LEVEL_DRAWS)} if dropout.threshold else {}
 
 
 # ---- one decoder level as ONE autograd node, without a single concat ---------------------------------------------------
@@ -411,13 +434,38 @@ def _raw_bn_bwd(x, y, ld_y, srcs, q, stats, act):
     return gx, gg, gb
 
 
+def _level_norm(P, groups, masks):
+    """norm(name, x, act, y, ld_y): the normaliser (and activation, and mask) of the dense x into y, a tensor of its own or a channel
+    slice -> what its backward needs"""
+    if groups is None:
+        return lambda name, x, act, y, ld_y: _raw_bn(x, P[name], act, y, ld_y)
+    from . import norm as N
+
+    def norm(name, x, act, y, ld_y):
+        plan = N._plan(x.shape, x.dtype, groups)
+        return plan, N._raw_gn(plan, x, x.shape[-1], P[name]["gamma"], P[name]["beta"], N.GN_EPSILON, act, masks.get(name), y, ld_y, True)
+    return norm
+
+
+def _level_norm_bwd(P, st, groups, masks):
+    """norm_bwd(name, x, y, ld_y, srcs, act) -> (dL/dx, dL/dgamma, dL/dbeta)"""
+    if groups is None:
+        return lambda name, x, y, ld_y, srcs, act: _raw_bn_bwd(x, y, ld_y, srcs, P[name], st[name], act)
+    from . import norm as N
+
+    def norm_bwd(name, x, y, ld_y, srcs, act):  # (y is not read: the kernels form it again)
+        plan, buf = st[name]
+        return N._raw_gn_bwd(plan, x, x.shape[-1], srcs, P[name]["gamma"], P[name]["beta"], buf, act, masks.get(name))
+    return norm_bwd
+
+
 _LEVEL_CONVS = ("up", "sup", "aspp_up", "aspp_up2", "skip", "skip2", "out")
 
 
 class _DenseLevel(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, concat, skip_feat, skip2, *flat):
-        names, rates, use_skip, use_skip2, extras = cfg
+        names, rates, use_skip, use_skip2, extras, groups, masks = cfg
         ctx.set_materialize_grads(False)
         # name -> dict(w, gamma, beta) / dict(gamma, beta) for 'skip_bn', plus the moving statistics (not differentiated)
         P, k = {}, 0
@@ -430,36 +478,38 @@ class _DenseLevel(torch.autograd.Function):
         dims = (B, H, W)
         C = P["sup"]["w"].shape[3]
         nC = (5 if use_skip2 else 4) * C
+        norm = _level_norm(P, groups, masks)
         with torch.cuda.device(concat.device):
             u0 = _raw_resize(concat, H, W)                                                      # :454
             a_up = _raw_conv(u0, u0.shape[3], P["up"]["w"], dims, 0)                            # :455
             upnet = torch.empty_like(a_up)
-            st = {"up": _raw_bn(a_up, P["up"], 0, upnet, upnet.shape[3])}
+            st = {"up": norm("up", a_up, 0, upnet, upnet.shape[3])}
             X = torch.empty(B, H, W, nC, dtype=torch.float32, device=concat.device)            # the level's ONE concat buffer
             sl = lambda a, b: X[..., a * C:b * C]                                               # noqa: E731  (views: pointers only)
             a_sup = _raw_conv(upnet, upnet.shape[3], P["sup"]["w"], dims, 0)                    # :456
-            st["sup"] = _raw_bn(a_sup, P["sup"], 1, sl(0, 1), nC)
+            st["sup"] = norm("sup", a_sup, 1, sl(0, 1), nC)
             a_au = _raw_conv(upnet, upnet.shape[3], P["aspp_up"]["w"], dims, rates[0])          # :457
-            st["aspp_up"] = _raw_bn(a_au, P["aspp_up"], 1, sl(1, 2), nC)
+            st["aspp_up"] = norm("aspp_up", a_au, 1, sl(1, 2), nC)
             a_au2 = _raw_conv(sl(0, 2), nC, P["aspp_up2"]["w"], dims, rates[1])                 # :458 reads [supnet, aspp_up]
-            st["aspp_up2"] = _raw_bn(a_au2, P["aspp_up2"], 1, sl(2, 3), nC)
+            st["aspp_up2"] = norm("aspp_up2", a_au2, 1, sl(2, 3), nC)
             sk = None
             if use_skip:
                 sk = torch.empty_like(skip_feat)
-                st["skip_bn"] = _raw_bn(skip_feat, P["skip_bn"], 1, sk, sk.shape[3])            # :460
+                st["skip_bn"] = norm("skip_bn", skip_feat, 1, sk, sk.shape[3])            # :460
                 a_sk = _raw_conv(sk, sk.shape[3], P["skip"]["w"], dims, 0)                      # :461
             else:
                 a_sk = _raw_conv(sl(1, 3), nC, P["skip"]["w"], dims, rates[1] * 2)              # :463 reads [aspp_up, aspp_up2]
-            st["skip"] = _raw_bn(a_sk, P["skip"], 1, sl(3, 4), nC)
+            st["skip"] = norm("skip", a_sk, 1, sl(3, 4), nC)
             s2 = a_s2 = None
             if use_skip2:
                 s2 = _raw_resize(skip2, H, W)                                                   # :465
                 a_s2 = _raw_conv(s2, s2.shape[3], P["skip2"]["w"], dims, 0)                     # :466
-                st["skip2"] = _raw_bn(a_s2, P["skip2"], 1, sl(4, 5), nC)
+                st["skip2"] = norm("skip2", a_s2, 1, sl(4, 5), nC)
             a_out = _raw_conv(X, nC, P["out"]["w"], dims, 0)                                    # :470 reads the whole buffer
             xconcat = torch.empty_like(a_out)
-            st["out"] = _raw_bn(a_out, P["out"], 0, xconcat, C)
+            st["out"] = norm("out", a_out, 0, xconcat, C)
         ctx.cfg, ctx.P, ctx.st = cfg, P, st
+        ctx.drawn = [(m.rng, m.rng._version) for m in masks.values() if m.rng is not None]
         ctx.acts = (u0, a_up, a_sup, a_au, a_au2, sk, a_sk, s2, a_s2, X, a_out)
         ctx.io = (concat.shape, skip2.shape if use_skip2 else None)
         ctx.save_for_backward(xconcat, upnet, *([skip_feat] if use_skip else []))
@@ -467,8 +517,12 @@ class _DenseLevel(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_x, g_up):
-        names, rates, use_skip, use_skip2, _ = ctx.cfg
+        names, rates, use_skip, use_skip2, _, groups, masks = ctx.cfg
         P, st = ctx.P, ctx.st
+        if any(rng._version != v for rng, v in ctx.drawn):
+            raise RuntimeError("the (seed, step) tensor of the level's dropout has been modified by an inplace operation since its "
+                               "forward: advance the step when its backward is done")
+        norm_bwd = _level_norm_bwd(P, st, groups, masks)
         xconcat, upnet = ctx.saved_tensors[:2]
         skip_feat = ctx.saved_tensors[2] if use_skip else None
         u0, a_up, a_sup, a_au, a_au2, sk, a_sk, s2, a_s2, X, a_out = ctx.acts
@@ -481,34 +535,34 @@ class _DenseLevel(torch.autograd.Function):
             if g_x is None:
                 g_x = torch.zeros_like(xconcat)
             g_x = g_x.contiguous()
-            g_a, G["out.gamma"], G["out.beta"] = _raw_bn_bwd(a_out, xconcat, C, [(g_x, C)], P["out"], st["out"], 0)
+            g_a, G["out.gamma"], G["out.beta"] = norm_bwd("out", a_out, xconcat, C, [(g_x, C)], 0)
             gX, G["out.w"] = _raw_conv_bwd(X, nC, P["out"]["w"], g_a, dims, 0)                  # dL/d(concat buffer), one piece
             gsl = lambda a: (gX[..., a * C:(a + 1) * C], nC)                                    # noqa: E731
             ysl = lambda a: X[..., a * C:(a + 1) * C]                                           # noqa: E731
             g_skip2 = None
             if use_skip2:
-                g_a, G["skip2.gamma"], G["skip2.beta"] = _raw_bn_bwd(a_s2, ysl(4), nC, [gsl(4)], P["skip2"], st["skip2"], 1)
+                g_a, G["skip2.gamma"], G["skip2.beta"] = norm_bwd("skip2", a_s2, ysl(4), nC, [gsl(4)], 1)
                 g_s2, G["skip2.w"] = _raw_conv_bwd(s2, s2.shape[3], P["skip2"]["w"], g_a, dims, 0)
                 g_skip2 = _raw_resize_bwd(g_s2, skip2_shape[1], skip2_shape[2])
-            g_a, G["skip.gamma"], G["skip.beta"] = _raw_bn_bwd(a_sk, ysl(3), nC, [gsl(3)], P["skip"], st["skip"], 1)
+            g_a, G["skip.gamma"], G["skip.beta"] = norm_bwd("skip", a_sk, ysl(3), nC, [gsl(3)], 1)
             g_skip_feat, t4 = None, None
             if use_skip:
                 g_sk, G["skip.w"] = _raw_conv_bwd(sk, sk.shape[3], P["skip"]["w"], g_a, dims, 0)
-                g_skip_feat, G["skip_bn.gamma"], G["skip_bn.beta"] = _raw_bn_bwd(skip_feat, sk, sk.shape[3], [(g_sk, sk.shape[3])],
-                                                                                P["skip_bn"], st["skip_bn"], 1)
+                g_skip_feat, G["skip_bn.gamma"], G["skip_bn.beta"] = norm_bwd("skip_bn", skip_feat, sk, sk.shape[3],
+                                                                              [(g_sk, sk.shape[3])], 1)
             else:
                 t4, G["skip.w"] = _raw_conv_bwd(ysl(1), nC, P["skip"]["w"], g_a, dims, rates[1] * 2)   # -> [aspp_up, aspp_up2]
             src = [gsl(2)] + ([(t4[..., C:], 2 * C)] if t4 is not None else [])
-            g_a, G["aspp_up2.gamma"], G["aspp_up2.beta"] = _raw_bn_bwd(a_au2, ysl(2), nC, src, P["aspp_up2"], st["aspp_up2"], 1)
+            g_a, G["aspp_up2.gamma"], G["aspp_up2.beta"] = norm_bwd("aspp_up2", a_au2, ysl(2), nC, src, 1)
             t5, G["aspp_up2.w"] = _raw_conv_bwd(ysl(0), nC, P["aspp_up2"]["w"], g_a, dims, rates[1])   # -> [supnet, aspp_up]
             src = [gsl(1), (t5[..., C:], 2 * C)] + ([(t4, 2 * C)] if t4 is not None else [])
-            g_a, G["aspp_up.gamma"], G["aspp_up.beta"] = _raw_bn_bwd(a_au, ysl(1), nC, src, P["aspp_up"], st["aspp_up"], 1)
+            g_a, G["aspp_up.gamma"], G["aspp_up.beta"] = norm_bwd("aspp_up", a_au, ysl(1), nC, src, 1)
             g_u1, G["aspp_up.w"] = _raw_conv_bwd(upnet, upnet.shape[3], P["aspp_up"]["w"], g_a, dims, rates[0])
-            g_a, G["sup.gamma"], G["sup.beta"] = _raw_bn_bwd(a_sup, ysl(0), nC, [gsl(0), (t5, 2 * C)], P["sup"], st["sup"], 1)
+            g_a, G["sup.gamma"], G["sup.beta"] = norm_bwd("sup", a_sup, ysl(0), nC, [gsl(0), (t5, 2 * C)], 1)
             g_u2, G["sup.w"] = _raw_conv_bwd(upnet, upnet.shape[3], P["sup"]["w"], g_a, dims, 0)
             Cu = upnet.shape[3]
             src = [(g_u1, Cu), (g_u2, Cu)] + ([(g_up.contiguous(), Cu)] if g_up is not None else [])
-            g_a, G["up.gamma"], G["up.beta"] = _raw_bn_bwd(a_up, upnet, Cu, src, P["up"], st["up"], 0)
+            g_a, G["up.gamma"], G["up.beta"] = norm_bwd("up", a_up, upnet, Cu, src, 0)
             g_u0, G["up.w"] = _raw_conv_bwd(u0, u0.shape[3], P["up"]["w"], g_a, dims, 0)
             g_concat = _raw_resize_bwd(g_u0, concat_shape[1], concat_shape[2])
         flat = []
@@ -518,7 +572,7 @@ class _DenseLevel(torch.autograd.Function):
         return (None, g_concat, g_skip_feat, g_skip2, *flat)
 
 
-def _check_level(params, concat, skip_feat, use_skip, use_skip2, skip2, need_moving=False):
+def _check_level(params, concat, skip_feat, use_skip, use_skip2, skip2, need_moving=False, groups=None):
     """argument checks of the concat-free level (the kernels index with these sizes and check nothing themselves) ->
     (names, flat parameter list, moving statistics per name, concat, skip_feat, skip2)"""
     names = [n for n in _LEVEL_CONVS if n != "skip2" or use_skip2] + (["skip_bn"] if use_skip else [])
@@ -560,14 +614,20 @@ def _check_level(params, concat, skip_feat, use_skip, use_skip2, skip2, need_mov
         _same_device(concat, *([q["w"]] if nm != "skip_bn" else []), *tensors.values())
         flat += vecs if nm == "skip_bn" else [q["w"], *vecs]
         extras[nm] = {k: q[k] for k in ("moving_mean", "moving_var") if q.get(k) is not None}
+        if groups is not None and (int(groups) < 1 or cv % int(groups)):
+            raise ValueError(f"groups must divide the {cv} channels of {nm}, got {groups}")
         if need_moving and len(extras[nm]) != 2:
             raise ValueError(f"is_training=False needs {nm}.moving_mean and {nm}.moving_var")
     return names, flat, extras, concat, skip_feat, skip2
 
 
-def _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2):
-    names, flat, extras, concat, skip_feat, skip2 = _check_level(params, concat, skip_feat, use_skip, use_skip2, skip2)
-    cfg = (tuple(names), tuple(int(r) for r in rates), bool(use_skip), bool(use_skip2), extras)
+def _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2, groups=None, masks={}):
+    names, flat, extras, concat, skip_feat, skip2 = _check_level(params, concat, skip_feat, use_skip, use_skip2, skip2, groups=groups)
+    if masks:
+        from .norm import _check_mask
+        for m in masks.values():
+            _check_mask(m, concat)
+    cfg = (tuple(names), tuple(int(r) for r in rates), bool(use_skip), bool(use_skip2), extras, groups, masks)
     return _DenseLevel.apply(cfg, concat, skip_feat if use_skip else None, skip2 if use_skip2 else None, *flat)
 
 
@@ -626,7 +686,7 @@ def _dense_level_infer(params, concat, skip_feat, rates, use_skip, use_skip2, sk
 
 def disp_bottleneck_dense(params: dict, concat: Tensor, skip_feat: Tensor = None, rates=(2, 4), use_skip: bool = True,
                           use_skip2: bool = True, skip2: Tensor = None, process_group=None, fused_level: bool = True,
-                          is_training: bool = True):
+                          is_training: bool = True, groups: int = None, dropout=None):
     """``nets.disp_bottleneck_dense`` (nets.py:451-471), one decoder level of ``disp_aspp_u_dense``, every op a
     hand-written kernel: x2 bilinear upsample, 1x1 and dilated 3x3 convolutions on fp32 MFMA, batch norm (training) +
     ELU.  ``fused_level`` (default; single-rank statistics only): the level is ONE autograd node that never materialises
@@ -639,15 +699,28 @@ def disp_bottleneck_dense(params: dict, concat: Tensor, skip_feat: Tensor = None
     'up' (:455), 'sup' (:456), 'aspp_up' (:457), 'aspp_up2' (:458), 'skip' (:461 or :463), ['skip2' (:466)], 'out'
     (:470) and, with use_skip, 'skip_bn' = dict(gamma, beta, ...) for the batch norm of the skip feature (:460).
     ``skip_feat`` = end_points[skip_block].  Returns (xconcat, upnet) like the reference.  ``process_group``: every
-    batch norm of the block takes its statistics over all ranks of the group (see ``batch_norm_elu``)."""
+    batch norm of the block takes its statistics over all ranks of the group (see ``batch_norm_elu``).
+
+    ``groups`` (not in the reference): every normaliser of the block is a group norm of that many groups (``group_norm_act``) with the
+    same gamma and beta, in training and in serving alike; moving statistics are neither read nor updated, and a ``process_group``
+    has nothing to exchange.  ``dropout``: a ``DropoutMask`` for the activated convolutions 'sup', 'aspp_up', 'aspp_up2', 'skip', 'skip2'
+    (layers mask.layer ... mask.layer + 4, a draw each); it is the epilogue of the group norm, an operator of its own behind a
+    batch norm (then the operators are composed through autograd), and ignored with ``is_training=False``."""
     from .pyramid import resize_bilinear
     import functools
     import os
-    if not is_training:
+    groups = None if groups is None else int(groups)
+    masks = _level_masks(dropout) if is_training else {}
+    if not is_training and groups is None:
         return _dense_level_infer(params, concat, skip_feat, rates, use_skip, use_skip2, skip2)
-    if process_group is None and fused_level and os.environ.get("SFM_LEVEL_FUSED", "1") != "0":
-        return _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2)
-    conv = functools.partial(_slim_conv, process_group=process_group)
+    if not is_training:
+        with torch.no_grad():
+            return _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2, groups)
+    if groups is not None:
+        process_group = None
+    if process_group is None and fused_level and os.environ.get("SFM_LEVEL_FUSED", "1") != "0" and not (masks and groups is None):
+        return _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2, groups, masks)
+    conv = functools.partial(_slim_conv, process_group=process_group, groups=groups, masks=masks)
     h, w = concat.shape[1], concat.shape[2]
     upnet = resize_bilinear(concat, 2 * h, 2 * w)                                        # :454
     upnet = conv(upnet, params, "up", activation=False)                            # :455
@@ -656,8 +729,7 @@ def disp_bottleneck_dense(params: dict, concat: Tensor, skip_feat: Tensor = None
     aspp_up2 = conv(torch.cat([supnet, aspp_up], dim=3), params, "aspp_up2", rate=rates[1])   # :458
     if use_skip:
         q = params["skip_bn"]
-        skip = batch_norm_elu(skip_feat, q["gamma"], q["beta"], q.get("moving_mean"), q.get("moving_var"),
-                              process_group=process_group)                               # :460
+        skip = _normalise(skip_feat, q, True, process_group, groups, None)               # :460
         skip = conv(skip, params, "skip")                                          # :461
     else:
         skip = conv(torch.cat([aspp_up, aspp_up2], dim=3), params, "skip", rate=rates[1] * 2)   # :463
@@ -720,7 +792,8 @@ def disp_head(x: Tensor, w: Tensor, b: Tensor) -> Tensor:
     return _DispHead.apply(x, w, b)
 
 
-def disp_aspp_u_dense_decoder(end_points: dict, params: dict, process_group=None, is_training: bool = True):
+def disp_aspp_u_dense_decoder(end_points: dict, params: dict, process_group=None, is_training: bool = True, groups: int = None,
+                              dropout=None):
     """The decoder of ``nets.disp_aspp_u_dense`` (nets.py:666-692) from the ResNet end-points to the three disparity
     maps - everything of the network that is not the stock ResNet-v2-50 encoder: batch norm + ELU + 1x1 on block4
     (:672-673), the five ``disp_bottleneck_dense`` levels (:675-686) and the three heads (:678, 683, 689).
@@ -732,9 +805,16 @@ def disp_aspp_u_dense_decoder(end_points: dict, params: dict, process_group=None
     parameter dicts of ``disp_bottleneck_dense``, 'disp2', 'disp3', 'disp4' = dict(w [3,3,C,1], b [1]).
     Returns ``[disp4, disp3, disp2]`` like the reference ([B,32h,32w,1], [B,16h,16w,1], [B,8h,8w,1]).
     ``is_training=False`` (test_kitti_depth_con.py:19-65; ``moving_mean`` / ``moving_var`` in every batch-norm dict): the
-    serving path - forward only, no autograd graph, one kernel pass per ``slim.conv2d``, no concat."""
+    serving path - forward only, no autograd graph, one kernel pass per ``slim.conv2d``, no concat.
+    ``groups``, ``dropout``: group norm in the place of every batch norm, and a ``DropoutMask`` for the levels' activations (level k
+    draws at layers mask.layer + 8 k ...; see ``disp_bottleneck_dense``); with ``groups`` the serving path needs no moving statistics."""
     q = params["stem_bn"]
-    if not is_training:
+    _level_masks(dropout)  # (its type)
+    if groups is not None:
+        with contextlib.nullcontext() if is_training else torch.no_grad():
+            upnet = _normalise(end_points["block4"], q, True, None, groups, None)                            # :672
+            upnet = _slim_conv(upnet, params, "stem", activation=False, groups=groups)                       # :673
+    elif not is_training:
         x4 = _check(end_points["block4"], "block4", 4)
         for nm in ("stem_bn", "stem"):
             if params[nm].get("moving_mean") is None or params[nm].get("moving_var") is None:
@@ -750,9 +830,12 @@ def disp_aspp_u_dense_decoder(end_points: dict, params: dict, process_group=None
         upnet = batch_norm_elu(end_points["block4"], q["gamma"], q["beta"], q.get("moving_mean"), q.get("moving_var"),
                                process_group=process_group)                                                  # :672
         upnet = _slim_conv(upnet, params, "stem", activation=False, process_group=process_group)             # :673
-    lvl = lambda name, x, skip, **kw: disp_bottleneck_dense(params[name], x, skip, process_group=process_group,  # noqa: E731
-                                                            is_training=is_training, **kw)
-    import contextlib
+    level_of = {name: k for k, (name, *_) in enumerate(DECODER_LEVELS)}
+
+    def lvl(name, x, skip, **kw):
+        mask = dropout.for_layer(dropout.layer + 8 * level_of[name]) if dropout is not None else None
+        return disp_bottleneck_dense(params[name], x, skip, process_group=process_group, is_training=is_training, groups=groups,
+                                     dropout=mask, **kw)
     with (contextlib.nullcontext() if is_training else torch.no_grad()):
         concat, _ = lvl("concat", upnet, end_points["block3"], use_skip2=False)                                  # :675
         concat1, skip1 = lvl("concat1", concat, end_points["block2"], use_skip2=False)                           # :676
