@@ -114,7 +114,7 @@ extern "C" int sfm_dropout(const void* x, int dtype, long long items, long long 
   if (items > 0xffffffffll - item0 || blocks > 0xffffffffll || (__int128)items * item_elems > ((__int128)1 << 60))
     return SFM_ERR_TOO_LARGE;
   const long long groups = (items * blocks + kPer * kBlock - 1) / (kPer * kBlock);
-  if (groups > 0x7fffffffll) return SFM_ERR_TOO_LARGE;
+  if (groups > kMaxGrid) return SFM_ERR_TOO_LARGE;
   const bool whole = item_elems % 8 == 0, away = far(2 * items * item_elems * es);
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

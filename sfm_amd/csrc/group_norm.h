@@ -327,13 +327,14 @@ static int gn_setup(long long B, long long N, int C, int G, int dtype, long long
                     dim3& last) {
   if (dtype < kF32 || dtype > kF16 || B < 1 || N < 1 || C < 1 || G < 1 || C % G || ld < C) return SFM_ERR_ARG;
   const int es = dtype == kF32 ? 4 : 2;
-  // items are counted in 32 bits, workgroups in 31, elements in 60 with room for strides; the rows that a workgroup takes at once
-  // lie within 31 bits of bytes of each other
+  // items are counted in 31 bits, elements in 60 with room for strides, the threads of a launch in 32 per dimension of the grid; the
+  // rows that a workgroup takes at once lie within 31 bits of bytes of each other
   if (B > 0x7fffffffll || (__int128)B * N > ((__int128)1 << 40) || ld > 0x7fffffffll / es || !gn_plan(B, N, C, G, es, backward, p))
     return SFM_ERR_TOO_LARGE;
   gn_tiles(p, (int)std::min<long long>(p.row_lanes, 0x7fffffffll / (ld * es)));
   const __int128 blocks = (__int128)B * p.slabs * std::max(p.first.chunks, p.last.chunks);
-  if (blocks + C > 0x7fffffffll || p.slabs > 65535) return SFM_ERR_TOO_LARGE;  // (with those that sum the parameters' gradients)
+  // (a launch's workgroups in one dimension, and with them those that sum the parameters' gradients; up to 1024 threads each)
+  if (blocks + C > kMaxGrid || p.slabs > 65535) return SFM_ERR_TOO_LARGE;
   first = dim3((unsigned)B, p.first.chunks, p.slabs);
   last = dim3((unsigned)B, p.last.chunks, p.slabs);
   return SFM_OK;

@@ -7,6 +7,8 @@
 
 namespace sfm {
 
+constexpr long long kMaxGrid = (1ll << 32) / 1024 - 1;  // workgroups of up to 1024 threads in a dimension of a grid
+
 // ---- element types (SFM_F32 / SFM_BF16 / SFM_F16 of the C ABI).  Everything is computed in fp32; a 16-bit tensor is rounded
 // once, to nearest even, where it is stored.
 enum { kF32 = 0, kBF16 = 1, kF16 = 2 };

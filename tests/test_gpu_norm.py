@@ -14,6 +14,7 @@ A 16-bit type's smallest step near zero (fp16: 2^-25 absolute) is added for valu
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import sfm_amd
 from oracle import norm_ref as R
@@ -69,6 +70,7 @@ SHAPES = [  # shape, groups: every vector width, whole and split groups, ragged 
     ((2, 19, 4096), 1), ((2, 19, 1028), 1), ((1, 9, 2500), 2), ((1, 11, 4100), 2),  # groups wider than a workgroup
     ((1000, 1, 24), 3), ((300, 5, 8), 1), ((70, 3, 3, 40), 40),     # many small items; one channel per group
     ((1, 5000, 8), 2), ((1, 4099, 20), 5), ((1, 257, 2048), 2048),
+    ((2, 300, 64), 64), ((2, 511, 32), 8), ((2, 512, 32), 8), ((2, 513, 32), 8), ((3, 130, 96), 2), ((1, 128, 1024), 1),  # about what a workgroup holds
 ]
 
 
@@ -197,6 +199,42 @@ def test_strides(dev):
     assert torch.equal(g1, g2)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("N,C,groups", [(37, 24, 4), (700, 32, 8), (5000, 20, 5), (65, 7, 7), (9, 2500, 2)])
+def test_slices_of_buffers(dev, N, C, groups, dtype):
+    """the C ABI as a level without concats calls it: x and y slices of wider buffers, nothing beside the slices written, dL/dy the
+    sum of three slices with strides of their own"""
+    import ctypes
+    from sfm_amd import _lib
+    from sfm_amd._lib import ptr, stream_of
+    B, act = 2, 1
+    x, gy, gamma, beta = inputs((B, N, C), dtype, 55, dev)
+    want = R.group_norm_act(f64(x), f64(gamma), f64(beta), groups, 1e-5, "elu", f64(gy))
+    wx, wy = torch.full((B, N, C + 11), 7.0, device=dev, dtype=dtype), torch.full((B, N, C + 5), 7.0, device=dev, dtype=dtype)
+    wx[..., 3:3 + C] = x
+    parts = [torch.full((B, N, C + k), 5.0, device=dev, dtype=dtype) for k in (1, 4, 0)]
+    halves = [(gy.float() * f).to(dtype) for f in (0.5, 0.25)]
+    for p, v in zip(parts, (*halves, (gy.float() - halves[0].float() - halves[1].float()).to(dtype))):
+        p[..., p.shape[-1] - C:] = v                      # powers of two and an exact rest: the sum is gy again
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    lib, es = _lib.load(), x.element_size()
+    mean, rstd = (torch.empty(B, groups, device=dev) for _ in range(2))
+    ws = torch.empty(lib.sfm_group_norm_workspace_floats(B, N, C, groups, code, 1) + 2, device=dev)
+    no_mask = (None, 0, 0, 0, 0, 0, 0)
+    at = ctypes.c_void_p
+    rc = lib.sfm_group_norm_act_fwd(at(wx.data_ptr() + 3 * es), C + 11, code, ptr(gamma), ptr(beta), B, N, C, groups, 1e-5, act, *no_mask,
+                                    at(wy.data_ptr() + 2 * es), C + 5, ptr(mean), ptr(rstd), ptr(ws), stream_of(x))
+    assert rc == 0
+    assert (wy[..., :2] == 7).all() and (wy[..., 2 + C:] == 7).all()
+    gx, gg, gb = torch.empty_like(x), torch.empty(C, device=dev), torch.empty(C, device=dev)
+    srcs = (ctypes.c_void_p * 3)(*[p.data_ptr() + (p.shape[-1] - C) * es for p in parts])
+    lds = (ctypes.c_longlong * 3)(*[p.shape[-1] for p in parts])
+    rc = lib.sfm_group_norm_act_bwd(at(wx.data_ptr() + 3 * es), C + 11, code, srcs, lds, 3, ptr(gamma), ptr(beta), ptr(mean), ptr(rstd), B, N,
+                                    C, groups, act, *no_mask, ptr(gx), ptr(gg), ptr(gb), ptr(ws), stream_of(x))
+    assert rc == 0
+    compare(wy[..., 2:2 + C], (gx, gg, gb), want, dtype)
+
+
 def test_sizes_of_zero(dev):
     g = torch.ones(8, device=dev, requires_grad=True)
     for shape in ((0, 3, 8), (2, 0, 8), (0, 8)):
@@ -289,6 +327,48 @@ def test_seed_and_step_on_the_device(dev):
 
 
 # ---- how it is used
+def test_saved_tensors_elsewhere(dev):
+    """what is saved may come back as other tensors (here through the host), and a graph may be run twice"""
+    x, gy, gamma, beta = inputs((3, 200, 40), torch.float32, 99, dev)
+    mask = sfm_amd.DropoutMask(0.2, torch.tensor([4, 4], device=dev))
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    y = sfm_amd.group_norm_act(*leaves, 5, dropout=mask)
+    want = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, gy), want))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, gy)
+    with torch.autograd.graph.save_on_cpu():
+        y = sfm_amd.group_norm_act(*leaves, 5, dropout=mask)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, gy), want))
+    y = torch.utils.checkpoint.checkpoint(lambda *a: sfm_amd.group_norm_act(*a, 5, dropout=mask), *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, gy), want))
+
+
+def test_threads(dev):
+    """two Python threads, each on a stream of its own, forward and backward"""
+    import threading
+    x, gy, gamma, beta = inputs((4, 900, 48), torch.bfloat16, 102, dev)
+    mask = sfm_amd.DropoutMask(0.1, (1, 1))
+
+    def step():
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, gamma, beta)]
+        y = sfm_amd.group_norm_act(*leaves, 6, dropout=mask)
+        return (y.detach(), *torch.autograd.grad(y, leaves, gy))
+    want, got = step(), [None, None]
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[k] = [step() for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for runs in got for r in runs for a, b in zip(r, want))
+
+
 def test_reproducible(dev):
     x, gy, gamma, beta = inputs((4, 500, 48), torch.float32, 101, dev)
     mask = sfm_amd.DropoutMask(0.1, (1, 1))

@@ -117,7 +117,7 @@ def test_forward_refuses(kw):
     assert _fwd(**kw) == -1
 
 
-@pytest.mark.parametrize("kw", [dict(B=2 ** 31), dict(N=2 ** 40), dict(threshold=9, N=2 ** 33), dict(threshold=9, item0=2 ** 32 - 1)],
+@pytest.mark.parametrize("kw", [dict(B=2 ** 31), dict(B=2 ** 22), dict(N=2 ** 40), dict(ld_x=2 ** 29), dict(ld_y=2 ** 29), dict(C=2 ** 22, G=2 ** 20, ld_x=2 ** 22, ld_y=2 ** 22), dict(threshold=9, N=2 ** 33), dict(threshold=9, item0=2 ** 32 - 1)],
                          ids=lambda kw: ",".join(kw))
 def test_forward_refuses_what_its_counters_do_not_hold(kw):
     assert _fwd(**kw) == -2
@@ -148,7 +148,8 @@ def _drop(**kw):
 @pytest.mark.parametrize("kw,rc", [(dict(x=None), -1), (dict(y=None), -1), (dict(dtype=3), -1), (dict(items=0), -1), (dict(elems=0), -1),
                                    (dict(C=0), -1), (dict(C=7), -1), (dict(x=F + 2), -1), (dict(y=F + 1, dtype=1), -1),
                                    (dict(threshold=65536), -1), (dict(threshold=-1), -1), (dict(rng=F + 4), -1),
-                                   (dict(items=2 ** 32, item0=1), -2), (dict(elems=2 ** 38), -2)], ids=lambda v: str(v))
+                                   (dict(items=2 ** 32, item0=1), -2), (dict(elems=2 ** 38), -2),
+                                   (dict(items=2 ** 31, elems=16), -2), (dict(items=2 ** 20, elems=2 ** 41), -2)], ids=lambda v: str(v))
 def test_dropout_refuses(kw, rc):
     assert _drop(**kw) == rc
 
