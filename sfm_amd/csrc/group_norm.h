@@ -26,24 +26,26 @@ namespace {
 // kernels' bounds hold their registers down to that): one more than fits is a second round of the whole length.  Measured at 0.5 GB
 // a tensor, us: statistics at 4 / 6 / 8: 97 / 94 / 98; forward's last pass fp32 at 4 / 6: 180 / 171, bf16 at 4 / 6: 193 / 200; backward's sums fp32 at 4 / 5: 194 / 172
 // (16-bit types hold two vectors of eight in registers: 4); its last pass fp32 at 4 / 5: 251 / 245.
-constexpr int kWavesStats = 6;
-constexpr int waves_apply(int es) { return es == 4 ? 6 : 4; }
-constexpr int waves_sums(int es) { return es == 4 ? 5 : 4; }
-constexpr int waves_bwd_apply(int es) { return es == 4 ? 5 : 4; }
+// Vectors of up to four bytes take few registers and have few bytes in flight: more.
+constexpr int waves_stats(int es, int V) { return es * V <= 4 ? 8 : 6; }
+constexpr int waves_apply(int es, int V) { return es * V <= 4 || es == 4 ? 6 : 4; }
+constexpr int waves_sums(int es, int V) { return es * V <= 4 ? 8 : es == 4 ? 5 : 4; }
+constexpr int waves_bwd_apply(int es, int V) { return es * V <= 4 ? 6 : es == 4 ? 5 : 4; }
 // (a vector that crosses many groups has a set of statistics for each and takes what registers it needs)
 constexpr int bound_of(int groups_of_vector, int waves) { return groups_of_vector <= 2 ? waves : 4; }
 constexpr int kCUs = 256;
 constexpr int kMaxChunks = 1024;
-constexpr int kU = 4;  // rows a thread has in flight
+// rows a thread has in flight: more of them where a channel count that 16 bytes do not divide makes its vectors shorter
+constexpr int batch_of(int vector_bytes) { return vector_bytes >= 16 ? 4 : 8; }
 
-// How an item is cut: channels into slabs (whole groups, or an even part of one wide group), rows into tiles of kU * row_lanes
-// rows, and the tiles in turn to the chunks (tile t to chunk t % chunks), one workgroup each.  In turn and not in runs: the
+// How an item is cut: channels into slabs (whole groups, or an even part of one wide group), rows into tiles of U * row_lanes
+// rows (U = batch_of), and the tiles in turn to the chunks (tile t to chunk t % chunks), one workgroup each.  In turn and not in runs: the
 // workgroups then move through memory side by side.  Passes over tensors of 512 MB, nontemporal: read + write 175 us in turn, 190 in
 // runs; two reads + write 263 and 283.
 struct GnPlan {
   long long N;
   int C, G, cpg;
-  int V;                 // elements per thread and row
+  int V, U;              // elements per thread and row; rows in a batch of a thread
   int cs;                // channels of a slab (the last one of a group or of the row may have fewer)
   int slabs;             // slabs of a row
   int groups_per_slab;   // >= 1; 1 where a group has parts
@@ -73,7 +75,7 @@ static inline int gcd_int(int a, int b) {
 // (also once the numbers of chunks are known: a row stride may ask for fewer row lanes, which makes more tiles of the same chunks)
 static void gn_tiles(GnPlan& p, int row_lanes) {
   p.row_lanes = row_lanes;
-  p.tile_rows = kU * row_lanes;
+  p.tile_rows = p.U * row_lanes;
   p.tiles = (p.N + p.tile_rows - 1) / p.tile_rows;
   p.left = (int)(p.N - (p.tiles - 1) * p.tile_rows);
   for (GnPlan::Turn* t : {&p.first, &p.last}) {
@@ -98,12 +100,17 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, bool backwar
     if (p.cpg % p.V == 0) break;
     if (p.cpg / gcd_int(p.cpg, p.V) <= kBlock) break;
   }
+  p.U = batch_of(p.V * es);
   const int unit_groups = p.V / gcd_int(p.cpg, p.V);                      // groups of the smallest slab
   const long long unit = (long long)p.cpg * unit_groups;
   if (unit / p.V <= kBlock) {
-    long long k = 1;  // at least 128 bytes of a row, so that a slab's lines are its own
-    while (k * unit * es < 128 && k * unit < C) ++k;
-    while (k > 1 && k * unit / p.V > kBlock) --k;
+    // The narrowest slab of whole 128-byte lines: fewer partials for a workgroup to join than with a wide one.  Where rows are no whole lines
+    // that would have workgroups all over the chip read each other's lines, so a slab is then as wide as a workgroup.
+    const long long widest = std::min<long long>(kBlock * (long long)p.V, C) / unit;
+    long long k = widest;
+    if ((long long)C * es % 128 == 0)
+      for (long long n = 1; n < widest; ++n)
+        if (n * unit * es % 128 == 0) { k = n; break; }
     p.groups_per_slab = k * unit_groups < G ? (int)k * unit_groups : G;
     p.cs = p.groups_per_slab * p.cpg;
     p.parts = 1;
@@ -128,8 +135,8 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, bool backwar
     const long long each = (p.tiles + chunks - 1) / chunks;  // as even as whole tiles allow
     return (int)((p.tiles + each - 1) / each);
   };
-  p.first.chunks = deal(backward ? waves_sums(es) : kWavesStats);
-  p.last.chunks = deal(backward ? waves_bwd_apply(es) : waves_apply(es));
+  p.first.chunks = deal(backward ? waves_sums(es, p.V) : waves_stats(es, p.V));
+  p.last.chunks = deal(backward ? waves_bwd_apply(es, p.V) : waves_apply(es, p.V));
   p.P = p.first.chunks * p.parts;
   gn_tiles(p, p.row_lanes);
   return true;
@@ -162,7 +169,7 @@ __device__ __forceinline__ Where where(const GnPlan& p, unsigned b, unsigned chu
   return w;
 }
 
-// A tile's rows go to the row lanes in kU steps: step u, row lane ry: row u * row_lanes + ry of the tile.  Everything here but
+// A tile's rows go to the row lanes in U steps: step u, row lane ry: row u * row_lanes + ry of the tile.  Everything here but
 // the thread's own place is uniform: the address of a load is a uniform pointer and a 32-bit offset of the thread (gn_setup
 // keeps the rows of a step within 31 bits of bytes).
 struct Lane {
@@ -178,14 +185,14 @@ struct Lane {
 __device__ __forceinline__ int group_in_slab(const GnPlan& p, int channel) {
   return p.parts > 1 ? 0 : p.cpg_inv ? (int)__umulhi((unsigned)channel, p.cpg_inv) : channel;
 }
-struct Tile {
+template <int U> struct Tile {
   long long index;
   int steps;  // steps in which row lane 0 has a row
   int last;   // rows of the last of them (1 .. row_lanes)
   bool full;
   __device__ __forceinline__ Tile(const GnPlan& p, long long i) : index(i) {
     full = i < p.tiles - 1 || p.left == p.tile_rows;
-    steps = full ? kU : (p.left + p.row_lanes - 1) / p.row_lanes;
+    steps = full ? U : (p.left + p.row_lanes - 1) / p.row_lanes;
     last = full ? p.row_lanes : p.left - (steps - 1) * p.row_lanes;
   }
   __device__ __forceinline__ bool valid(int u, int ry) const { return full || u < steps - 1 || (u == steps - 1 && ry < last); }
@@ -199,7 +206,7 @@ __device__ __forceinline__ long long last_tile(const GnPlan& p, const Where& w) 
 }
 
 template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, for tensors that no cache holds until they are read again (far())
-  static constexpr int kES = ElemBytes<DT>::value;
+  static constexpr int kES = ElemBytes<DT>::value, U = batch_of(V * kES);
   const char* base;
   long long step;      // bytes of the rows of a step
   unsigned off, lead;  // of this thread; lead: its row lane's share of it
@@ -209,15 +216,15 @@ template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, f
     lead = (unsigned)(l.ry * ld * kES);
     off = lead + (unsigned)(l.vx * V * kES);
   }
-  __device__ __forceinline__ const char* at(const Tile& t) const { return base + t.index * kU * step; }
+  __device__ __forceinline__ const char* at(const Tile<U>& t) const { return base + t.index * U * step; }
   // step u < steps of the tile at `a`; in its last step a row lane without a row reads row lane 0's
-  __device__ __forceinline__ Raw<DT, V> row(const char* a, const Tile& t, int u, int ry) const {
+  __device__ __forceinline__ Raw<DT, V> row(const char* a, const Tile<U>& t, int u, int ry) const {
     return load_raw<DT, V, NT>(a + u * step, off - (t.valid(u, ry) ? 0u : lead));
   }
-  __device__ __forceinline__ void load(const Tile& t, int ry, Raw<DT, V> (&raw)[kU]) const {
+  __device__ __forceinline__ void load(const Tile<U>& t, int ry, Raw<DT, V> (&raw)[U]) const {
     const char* a = at(t);
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < U; ++u)
       if (u < t.steps) raw[u] = row(a, t, u, ry);
   }
   __device__ __forceinline__ void store(const char* a, int u, const float (&f)[V]) const {

@@ -11,8 +11,8 @@ struct GySrc {
   long long ld[3];
   int n;
 };
-template <int DT, int V>
-__device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, const Where& w, const Lane& l, const Tile& t, int u,
+template <int DT, int V, int U>
+__device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, const Where& w, const Lane& l, const Tile<U>& t, int u,
                                             float (&g)[V]) {
   for (int k = 1; k < s.n; ++k) {  // uniform
     const Stream<DT, V> more(s.p[k], s.ld[k], p, w, l);
@@ -25,19 +25,19 @@ __device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, con
 
 // ---- backward, first launch: per_group [B][G][P] (sum gamma dz, sum gamma dz xhat), per_channel [C][B][chunks] (sum dz, sum dz xhat)
 template <int DT, int V, int E, bool DROP>
-__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::value))) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::value, V))) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                              const float* __restrict__ gamma, const float* __restrict__ beta,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
                                                              GnPlan p, int B, int act, Drop drop, float2* __restrict__ per_group,
                                                              float2* __restrict__ per_channel) {
-  constexpr int A = V / E;
+  constexpr int A = V / E, U = batch_of(V * ElemBytes<DT>::value);
   __shared__ float2 red[kBlock * V];
   const Where w = where(p, blockIdx.x, blockIdx.y, blockIdx.z);
   const Lane l(p, w, p.row_lanes);
   if (l.mine) {
     const Stream<DT, V> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l);
-    Tile t(p, w.chunk);
-    Raw<DT, V> xr[kU], gr[kU];
+    Tile<U> t(p, w.chunk);
+    Raw<DT, V> xr[U], gr[U];
     xs.load(t, l.ry, xr);
     gs.load(t, l.ry, gr);
     const int c = w.c0 + l.vx * V;
@@ -53,13 +53,13 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
     const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
     for (;;) {
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
+      for (int u = 0; u < U; ++u) {
         if (u >= t.steps || !t.valid(u, l.ry)) break;
         float f[V], g[V], z[V];
         unpack<DT, V>(xr[u], f);
         unpack<DT, V>(gr[u], g);
-        if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, l, t, u, g);
-        if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * kU + u) * row_places + place, row_places);
+        if (gy.n > 1) add_more_gy<DT, V, U>(gy, p, w, l, t, u, g);
+        if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
 #pragma unroll
         for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
         act_bwd<V>(g, z, act);
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
         for (int k = 0; k < V; ++k) { s1[k] += g[k]; s2[k] = __builtin_fmaf(g[k], f[k], s2[k]); }
       }
       if (t.index + p.first.chunks >= p.tiles) break;
-      t = Tile(p, t.index + p.first.chunks);
+      t = Tile<U>(p, t.index + p.first.chunks);
       xs.load(t, l.ry, xr);
       gs.load(t, l.ry, gr);
     }
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
 // ---- backward, second launch: the first param_blocks workgroups sum the channel partials over items and chunks (a wave per
 // channel), the others write gx
 template <int DT, int V, int E, bool DROP, bool FAR>
-__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<DT>::value))) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<DT>::value, V))) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
                                                               GnPlan p, int B, int act, Drop drop,
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
                                                               const float2* __restrict__ per_channel, unsigned param_blocks,
                                                               void* __restrict__ gx, float* __restrict__ ggamma,
                                                               float* __restrict__ gbeta) {
-  constexpr int A = V / E;
+  constexpr int A = V / E, U = batch_of(V * ElemBytes<DT>::value);
   __shared__ float2 stat[kBlock * A];
   if (blockIdx.x < param_blocks) {
     const int c = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -137,8 +137,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
   const Where w = where(p, bid - rest * B, rest % (unsigned)p.last.chunks, rest / (unsigned)p.last.chunks);
   const Lane l(p, w, p.row_lanes);
   const Stream<DT, V, FAR> xs(x, ldx, p, w, l), gs(gy.p[0], gy.ld[0], p, w, l), os(gx, p.C, p, w, l);
-  Tile t(p, FAR ? w.chunk : last_tile(p, w));
-  Raw<DT, V> xr[kU], gr[kU];
+  Tile<U> t(p, FAR ? w.chunk : last_tile(p, w));
+  Raw<DT, V> xr[U], gr[U];
   const int c = w.c0 + l.vx * V;
   float mu[A], is[A], ga[V], be[V], c1[A], c2[A];
   if (l.mine) {
@@ -177,13 +177,13 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
   for (;;) {
     const char* o = os.at(t);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (u >= t.steps) break;
       float f[V], g[V], z[V];
       unpack<DT, V>(xr[u], f);
       unpack<DT, V>(gr[u], g);
-      if (gy.n > 1) add_more_gy<DT, V>(gy, p, w, l, t, u, g);
-      if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * kU + u) * row_places + place, row_places);
+      if (gy.n > 1) add_more_gy<DT, V, U>(gy, p, w, l, t, u, g);
+      if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
 #pragma unroll
       for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
       act_bwd<V>(g, z, act);
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
       if (t.valid(u, l.ry)) os.store(o, u, g);
     }
     if (FAR ? t.index + p.last.chunks >= p.tiles : t.index < p.last.chunks) break;
-    t = Tile(p, FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
+    t = Tile<U>(p, FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
     xs.load(t, l.ry, xr);
     gs.load(t, l.ry, gr);
   }

@@ -35,9 +35,9 @@ __device__ __forceinline__ void reduce_stats(const float2* red, int lanes, int r
 
 // ---- forward, first launch: part [B][G][P] (mean, M2).  A thread has one pair for E adjacent channels of a group.
 template <int DT, int V, int E>
-__global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_stats(ElemBytes<DT>::value, V))) void gn_stats_kernel(const void* __restrict__ x, long long ldx, GnPlan p,
                                                           float2* __restrict__ part) {
-  constexpr int A = V / E;                   // accumulators
+  constexpr int A = V / E, U = batch_of(V * ElemBytes<DT>::value); // accumulators
   __shared__ float2 red[kBlock * A];         // [row lane][E channels of the slab]
   const Where w = where(p, blockIdx.x, blockIdx.y, blockIdx.z);
   const Lane l(p, w, p.row_lanes);
@@ -78,13 +78,13 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats
       n = nn;
     };
     for (long long i = w.chunk; i < p.tiles; i += p.first.chunks) {
-      const Tile t(p, i);
-      Raw<DT, V> raw[kU];
+      const Tile<U> t(p, i);
+      Raw<DT, V> raw[U];
       xs.load(t, l.ry, raw);
-      if (t.full) join(std::integral_constant<int, kU>{}, raw);
+      if (t.full) join(std::integral_constant<int, U>{}, raw);
       else {
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+        for (int u = 0; u < U; ++u)
           if (t.valid(u, l.ry)) join(std::integral_constant<int, 1>{}, raw + u);
       }
     }
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, kWavesStats)) void gn_stats
   __syncthreads();
   const bool partial = w.chunk == p.first.owner && p.left < p.tile_rows;
   const long long whole = p.first.own + (w.chunk < p.first.extra) - partial;   // whole tiles of this chunk
-  const int per_lane = (int)whole * kU + (partial ? p.left / p.row_lanes : 0), more = partial ? p.left % p.row_lanes : 0;
+  const int per_lane = (int)whole * U + (partial ? p.left / p.row_lanes : 0), more = partial ? p.left % p.row_lanes : 0;
   reduce_stats<kBlock, A, E>(red, p.lanes, p.row_lanes, per_lane, more, p.parts == 1 ? p.cpg : w.cc, w.ng, [&](int j, float mean, float m2) {
     part[((long long)w.b * p.G + w.g0 + j) * p.P + w.chunk * p.parts + w.part] = make_float2(mean, m2);
   });
@@ -155,18 +155,18 @@ template <int K> __device__ __forceinline__ void join_stats(const float2* __rest
 // ---- forward, second launch.  The first batch is on its way while the partials are joined; where a cache may still hold what the
 // first launch read last, the tiles go backwards (last_tile).
 template <int DT, int V, int E, bool DROP, bool FAR>
-__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::value))) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
+__global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::value, V))) void gn_apply_kernel(const void* __restrict__ x, long long ldx,
                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
                                                           const float2* __restrict__ part, GnPlan p, float eps, int act, Drop drop,
                                                           void* __restrict__ y, long long ldy, float* __restrict__ save_mean,
                                                           float* __restrict__ save_r) {
-  constexpr int A = V / E;
+  constexpr int A = V / E, U = batch_of(V * ElemBytes<DT>::value);
   __shared__ float2 stat[kBlock * A];
   const Where w = where(p, blockIdx.x, blockIdx.y, blockIdx.z);
   const Lane l(p, w, p.row_lanes);
   const Stream<DT, V, FAR> xs(x, ldx, p, w, l), ys(y, ldy, p, w, l);
-  Tile t(p, FAR ? w.chunk : last_tile(p, w));
-  Raw<DT, V> raw[kU];
+  Tile<U> t(p, FAR ? w.chunk : last_tile(p, w));
+  Raw<DT, V> raw[U];
   float sc[V], sh[V];
   const int c = w.c0 + l.vx * V;
   if (l.mine) {
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
 #pragma unroll
     for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k]; sh[k] = beta[c + k]; }
   }
-  join_stats<DT == kF32 ? 2 : 4>(part, p, w, eps, stat);
+  join_stats<V == 8 ? 4 : 2>(part, p, w, eps, stat);
   if (save_mean && w.chunk == 0 && w.part == 0)
     for (int j = threadIdx.x; j < w.ng; j += kBlock) {
       save_mean[(long long)w.b * p.G + w.g0 + j] = stat[j].x;
@@ -193,10 +193,10 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
   const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
   for (;;) {
     const bool more = FAR ? t.index + p.last.chunks < p.tiles : t.index >= p.last.chunks;
-    const Tile next(p, !more ? t.index : FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
+    const Tile<U> next(p, !more ? t.index : FAR ? t.index + p.last.chunks : t.index - p.last.chunks);
     const char *a = xs.at(next), *o = ys.at(t);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (u >= t.steps) break;
       float f[V];
       unpack<DT, V>(raw[u], f);
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
       act_fwd<V>(f, act);
-      if constexpr (DROP) mask.apply(f, u, (unsigned long long)(t.index * kU + u) * row_places + place, row_places);
+      if constexpr (DROP) mask.apply(f, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
       if (t.valid(u, l.ry)) ys.store(o, u, f);
     }
     if (!more) break;
