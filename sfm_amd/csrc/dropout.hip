@@ -11,12 +11,21 @@ constexpr int kPer = 4;  // blocks of eight elements a thread draws for; a workg
 __device__ __forceinline__ unsigned keep_eight(const Drop& d, const DropKey& key, unsigned item, unsigned blk, unsigned C) {
   if (!d.per_channel) return keep_bits(d, key, d.item0 + item, (unsigned long long)blk * 8);
   if (C % 8 == 0) return keep_bits(d, key, d.item0 + item, blk % (C / 8) * 8);
-  unsigned keep = 0, c = (unsigned)((unsigned long long)blk * 8 % C), have = ~0u, eight = 0;  // they cross from row to row
-#pragma unroll 1
-  for (int e = 0; e < 8; ++e) {
-    if ((c >> 3) != have) { have = c >> 3; eight = keep_bits(d, key, d.item0 + item, c & ~7u); }
-    keep |= ((eight >> (c & 7)) & 1u) << e;
-    c = c + 1 == C ? 0 : c + 1;
+  unsigned c = (unsigned)((unsigned long long)blk * 8 % C), keep = 0;  // they start anywhere in a row and cross into the next
+  if (C >= 8) {  // the rest of a block, the next one (or the row's first), and where the row ends with a short block one more
+    unsigned n = min(8 - (c & 7), C - c);
+    keep = (keep_bits(d, key, d.item0 + item, c) >> (c & 7)) & ((1u << n) - 1);
+    c = c + n == C ? 0 : c + n;
+    const unsigned more = min(8u, C - c);
+    keep |= (keep_bits(d, key, d.item0 + item, c) & ((1u << more) - 1)) << n;
+    n += more;
+    if (n < 8) keep |= keep_bits(d, key, d.item0 + item, c + more == C ? 0 : c + more) << n;
+  } else {
+    const unsigned all = keep_bits(d, key, d.item0 + item, 0);
+    for (int e = 0; e < 8; ++e) {
+      keep |= ((all >> c) & 1u) << e;
+      c = c + 1 == C ? 0 : c + 1;
+    }
   }
   return keep;
 }

@@ -64,6 +64,11 @@ def test_oracle_against_torch():
         np.testing.assert_allclose(R.group_norm_act(x, w, b, 4, 1e-5, kind)["y"], f(want).numpy(), rtol=1e-12, atol=1e-12)
 
 
+def test_autograd_module_is_built():
+    from sfm_amd import norm
+    assert callable(norm._nodes().group_norm_act) and callable(norm._nodes().dropout)
+
+
 # ---- refusals
 def test_cpu_tensors_are_rejected():
     x, g = torch.zeros(2, 3, 8), torch.ones(8)
