@@ -207,6 +207,11 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
       if constexpr (DROP) mask.apply(f, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
       if (t.valid(u, l.ry)) ys.store(o, u, f);
     }
+    if (!FAR && more && t.steps < U) {  // the item's last tile comes first where tiles go backwards; the next one has rows that it had not
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u >= t.steps && u < next.steps) raw[u] = xs.row(a, next, u, l.ry);
+    }
     if (!more) break;
     t = next;
   }

@@ -71,6 +71,8 @@ SHAPES = [  # shape, groups: every vector width, whole and split groups, ragged 
     ((1000, 1, 24), 3), ((300, 5, 8), 1), ((70, 3, 3, 40), 40),     # many small items; one channel per group
     ((1, 5000, 8), 2), ((1, 4099, 20), 5), ((1, 257, 2048), 2048),
     ((2, 300, 64), 64), ((2, 511, 32), 8), ((2, 512, 32), 8), ((2, 513, 32), 8), ((3, 130, 96), 2), ((1, 128, 1024), 1),  # about what a workgroup holds
+    # workgroups with several tiles of rows, the last tile short: the last pass starts with it (few rows, and one row lane's worth)
+    ((300, 1801, 32), 8), ((300, 1825, 32), 32), ((600, 700, 9), 3), ((500, 613, 36), 4),
 ]
 
 
@@ -122,6 +124,19 @@ def test_activations_and_masks(dev, shape, groups, dtype, p, per_channel, act):
     compare(y, grads, want, dtype, 65536 / (65536 - t), loose)
     if p:
         assert np.array_equal(f64(y) == 0, ~np.asarray(keep) | (want["y"] == 0))
+
+
+@pytest.mark.parametrize("per_channel", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape,groups", SHAPES[-4:], ids=["c32g8", "c32g32", "c9", "c36"])
+def test_masks_where_workgroups_take_several_tiles(dev, shape, groups, dtype, per_channel):
+    x, gy, gamma, beta = inputs(shape, dtype, 9, dev)
+    mask = sfm_amd.DropoutMask(0.4, (77, 3), layer=1, per_channel=per_channel, first_item=1)
+    keep = R.keep_mask(shape, mask.threshold, 77, 3, 1, per_channel, 1)
+    want = R.group_norm_act(f64(x), f64(gamma), f64(beta), groups, 1e-5, "elu", f64(gy), keep, mask.threshold)
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    y = sfm_amd.group_norm_act(*leaves, groups, activation="elu", dropout=mask)
+    compare(y, torch.autograd.grad(y, leaves, gy), want, dtype, 65536 / (65536 - mask.threshold))
 
 
 def test_gradient_against_differences(dev):
