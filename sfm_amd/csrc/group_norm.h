@@ -125,7 +125,7 @@ static bool gn_plan(long long B, long long N, int C, int G, int es, bool backwar
     p.slabs = G * p.parts;
   }
   p.lanes = p.cs / p.V;
-  p.pairs = p.V == 4 && es == 4 && C % 8 == 0 && p.cs % 8 == 0;
+  p.pairs = p.V == 4 && es == 4 && C % 8 == 0 && p.cs % 8 == 0 && (p.parts == 1 || p.cpg % 8 == 0);  // every slab starts and ends with a block
   p.lanes_inv = ((1u << 20) + p.lanes - 1) / p.lanes;
   p.cpg_inv = p.cpg == 1 ? 0u : (unsigned)(((1ull << 32) + p.cpg - 1) / p.cpg);
   gn_tiles(p, kBlock / p.lanes);

@@ -139,6 +139,21 @@ def test_masks_where_workgroups_take_several_tiles(dev, shape, groups, dtype, pe
     compare(y, torch.autograd.grad(y, leaves, gy), want, dtype, 65536 / (65536 - mask.threshold))
 
 
+@pytest.mark.parametrize("per_channel", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape,groups", [((2, 5, 2072), 2), ((3, 9, 2080), 2), ((2, 4, 6216), 6), ((2, 7, 1, 5140), 4)],
+                         ids=["parts520of1036", "parts520of1040", "parts520of1036x6", "parts of 1285"])
+def test_masks_where_a_group_has_parts(dev, shape, groups, dtype, per_channel):
+    """a part of a group may start in the middle of the mask's blocks of eight"""
+    x, gy, gamma, beta = inputs(shape, dtype, 13, dev)
+    mask = sfm_amd.DropoutMask(0.5, (91, 4), layer=2, per_channel=per_channel)
+    keep = R.keep_mask(shape, mask.threshold, 91, 4, 2, per_channel, 0)
+    want = R.group_norm_act(f64(x), f64(gamma), f64(beta), groups, 1e-5, "silu", f64(gy), keep, mask.threshold)
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    y = sfm_amd.group_norm_act(*leaves, groups, activation="silu", dropout=mask)
+    compare(y, torch.autograd.grad(y, leaves, gy), want, dtype, 65536 / (65536 - mask.threshold))
+
+
 def test_gradient_against_differences(dev):
     """directional differences of the fp32 kernel itself, at a step where the difference's own rounding (2 u |f| / step) and its
     curvature (step^2) are both under 1e-3 of the derivative"""
