@@ -169,6 +169,21 @@ void refuse_forward_mode(const char* name, const Tensor& t) {
   TORCH_CHECK(!t._fw_grad(0).defined(), name, " has no forward-mode derivative");
 }
 
+// A backward that is captured into a graph hands its gradients to the leaves on the stream on which autograd first met them.  While an
+// eager graph of the same leaves lives (or a hook on them) that is a stream outside the capture, which cannot be ended
+// then: the call is refused before anything of it is recorded.
+void refuse_foreign_leaf(const char* name, const Tensor& t, const Tensor& x) {
+  if (!t.requires_grad() || !t.is_leaf()) return;
+  const auto leaf = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!leaf) return;
+  const auto current = c10::hip::getCurrentHIPStream(x.get_device());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const auto met = leaf->stream();
+  TORCH_CHECK(!met.has_value() || *met == current.unwrap(), name, ": a stream capture, and a tensor that requires gradients and that autograd knows from "
+              "another stream: let go of what was computed from it outside of the capture (and of hooks on it), or give a detached copy");
+}
+
 template <typename NodeT, typename... T> std::shared_ptr<NodeT> make_node(const T&... inputs) {
   std::shared_ptr<NodeT> node(new NodeT(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
@@ -187,7 +202,10 @@ Tensor group_norm_act(const Tensor& x, const Tensor& gamma, const Tensor& beta, 
   s.N = s.B ? x.numel() / (s.B * s.C) : 0;
   Mask m{std::move(rng), seed, step, layer, item0, threshold, per_channel};
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || gamma.requires_grad() || beta.requires_grad());
-  for (const Tensor* t : {&x, &gamma, &beta}) refuse_forward_mode("group_norm_act", *t);
+  for (const Tensor* t : {&x, &gamma, &beta}) {
+    refuse_forward_mode("group_norm_act", *t);
+    if (grad) refuse_foreign_leaf("group_norm_act", *t, x);
+  }
   Tensor y, buf;
   {
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -228,12 +246,14 @@ Tensor dropout(const Tensor& x, std::optional<Tensor> rng, uint64_t seed, uint32
                bool per_channel) {
   Mask m{std::move(rng), seed, step, layer, item0, threshold, per_channel};
   refuse_forward_mode("dropout", x);
+  const bool grad = at::GradMode::is_enabled() && x.requires_grad();
+  if (grad) refuse_foreign_leaf("dropout", x, x);
   Tensor y;
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     y = run_dropout(x, m, m.rng.has_value() ? *m.rng : Tensor());
   }
-  if (at::GradMode::is_enabled() && x.requires_grad()) {
+  if (grad) {
     auto node = make_node<DropoutBackward>(x);
     if (m.rng.has_value()) node->rng_ = SavedVariable(*m.rng, false);
     node->m = std::move(m);

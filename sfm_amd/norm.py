@@ -25,6 +25,7 @@ Tensor = torch.Tensor
 GN_EPSILON = BN_EPSILON
 ACTIVATIONS = {None: 0, "none": 0, "elu": 1, "relu": 2, "silu": 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FP32 = torch.finfo(torch.float32)
 _autograd = None
 
 
@@ -52,6 +53,8 @@ def _check_activation(x, name: str) -> int:
         raise TypeError(f"{name} is on {x.device}; sfm_amd runs on ROCm devices only (no CPU fallback)")
     if x.dim() < 2:
         raise ValueError(f"{name} must be [B, ..., C] with at least two dimensions, got shape {tuple(x.shape)}")
+    if x.shape[-1] > 2 ** 31 - 1:
+        raise ValueError(f"{name} has {x.shape[-1]} channels, more than 2^31 - 1")
     return dt
 
 
@@ -222,8 +225,8 @@ def group_norm_act(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon:
     if not beta.is_contiguous():
         beta = beta.contiguous()
     epsilon = float(epsilon)
-    if not 0.0 < epsilon < float("inf"):
-        raise ValueError(f"epsilon must be positive and finite, got {epsilon}")
+    if not _FP32.tiny <= epsilon <= _FP32.max:
+        raise ValueError(f"epsilon must be positive and finite in float32, got {epsilon}")
     act = ACTIVATIONS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
     if act < 0:
         raise ValueError(f"activation must be one of {[a for a in ACTIVATIONS if a]} or None, got {activation!r}")

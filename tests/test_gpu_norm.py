@@ -460,6 +460,34 @@ def test_captured_step(dev):
     assert not torch.equal(seen[0] == 0, seen[1] == 0)
 
 
+def test_capture_refuses_leaves_that_an_eager_graph_holds(dev):
+    x, _, gamma, beta = inputs((2, 40, 32), torch.float32, 109, dev)
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    mask = sfm_amd.DropoutMask(0.2, (1, 2))
+    alive = sfm_amd.group_norm_act(*leaves, 4)
+    for call in (lambda: sfm_amd.group_norm_act(*leaves, 4), lambda: sfm_amd.group_norm_act(x.detach(), gamma, beta.detach(), 4),
+                 lambda: sfm_amd.dropout(x, mask)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = x.detach() + 1  # (a capture of nothing is warned of)
+            with pytest.raises(RuntimeError, match="stream capture"):
+                call()
+            with torch.no_grad():  # no backward: nothing is in the way
+                y = sfm_amd.group_norm_act(*leaves, 4)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, alive) and torch.equal(kept, x.detach() + 1)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(sfm_amd.group_norm_act(*leaves, 4).square().mean(), leaves)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(sfm_amd.group_norm_act(*leaves, 4).square().mean(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_gradients_are_born_in_the_buckets(dev):
     x, gy, gamma, beta = inputs((2, 40, 32), torch.float32, 107, dev)
     g, b = gamma.clone().requires_grad_(True), beta.clone().requires_grad_(True)
@@ -477,6 +505,7 @@ def test_refusals_with_device_tensors(dev):
     x, g = torch.zeros(2, 3, 8, device=dev), torch.ones(8, device=dev)
     for kw, err in ((dict(groups=3), ValueError), (dict(groups=0), ValueError), (dict(groups=16), ValueError),
                     (dict(groups=2, epsilon=0.0), ValueError), (dict(groups=2, epsilon=float("nan")), ValueError),
+                    (dict(groups=2, epsilon=1e-50), ValueError), (dict(groups=2, epsilon=1e39), ValueError),
                     (dict(groups=2, activation="gelu"), ValueError), (dict(groups=2, activation=True), ValueError),
                     (dict(groups=2, dropout=0.5), TypeError),
                     (dict(groups=2, dropout=sfm_amd.DropoutMask(0.1, (1, 2), first_item=2 ** 32 - 1)), ValueError)):
@@ -490,6 +519,8 @@ def test_refusals_with_device_tensors(dev):
         sfm_amd.group_norm_act(x, g.cpu(), g, 2)
     with pytest.raises(ValueError):
         sfm_amd.group_norm_act(g, g, g, 2)
+    with pytest.raises(ValueError, match="channels"):
+        sfm_amd.dropout(g[:1].expand(1, 2 ** 31), sfm_amd.DropoutMask(0.1, (1, 2)))
     with pytest.raises(TypeError):
         sfm_amd.dropout(x, 0.5)
     with pytest.raises(ValueError):
