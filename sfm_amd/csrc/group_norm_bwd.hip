@@ -41,27 +41,32 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
     xs.load(t, l.ry, xr);
     gs.load(t, l.ry, gr);
     const int c = w.c0 + l.vx * V;
-    float mu[A], is[A], ga[V], be[V], s1[V], s2[V];
+    float mu[A], is[A], sc[V], sh[V], s1[V], s2[V];  // s2: of dz (x - mean), which r makes sums of dz xhat in the end
 #pragma unroll
     for (int a = 0; a < A; ++a) {
       const long long g = (long long)w.b * p.G + w.g0 + group_in_slab(p, l.vx * V + a * E);
       mu[a] = mean[g]; is[a] = rstd[g];
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) { ga[k] = gamma[c + k]; be[k] = beta[c + k]; s1[k] = 0.0f; s2[k] = 0.0f; }
-  std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
+    for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k] * is[k / E]; sh[k] = beta[c + k]; s1[k] = 0.0f; s2[k] = 0.0f; }
+    std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
     const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
     for (;;) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (u >= t.steps || !t.valid(u, l.ry)) break;
+        if (u >= t.steps) break;
         float f[V], g[V], z[V];
         unpack<DT, V>(xr[u], f);
         unpack<DT, V>(gr[u], g);
         if (gy.n > 1) add_more_gy<DT, V, U>(gy, p, w, l, t, u, g);
         if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
+        if (!t.full) {  // a row lane without a row has read another's: nothing of it is added (a branch of its own would keep both ways' registers)
+          const bool counts = t.valid(u, l.ry);
 #pragma unroll
-        for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
+          for (int k = 0; k < V; ++k) g[k] = counts ? g[k] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) { f[k] -= mu[k / E]; z[k] = __builtin_fmaf(f[k], sc[k], sh[k]); }
         act_bwd<V>(g, z, act);
 #pragma unroll
         for (int k = 0; k < V; ++k) { s1[k] += g[k]; s2[k] = __builtin_fmaf(g[k], f[k], s2[k]); }
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
       gs.load(t, l.ry, gr);
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) red[l.ry * p.cs + l.vx * V + k] = make_float2(s1[k], s2[k]);
+    for (int k = 0; k < V; ++k) red[l.ry * p.cs + l.vx * V + k] = make_float2(s1[k], s2[k] * is[k / E]);
   }
   __syncthreads();
   // over the row lanes: S threads per channel take every S-th row lane each, then one adds the S.  In order: the same bits every time.
@@ -140,7 +145,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
   Tile<U> t(p, FAR ? w.chunk : last_tile(p, w));
   Raw<DT, V> xr[U], gr[U];
   const int c = w.c0 + l.vx * V;
-  float mu[A], is[A], ga[V], be[V], c1[A], c2[A];
+  float mu[A], is[A], sc[V], sh[V], c1[A], c2[A];
   if (l.mine) {
     xs.load(t, l.ry, xr);
     gs.load(t, l.ry, gr);
@@ -150,7 +155,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
       mu[a] = mean[g]; is[a] = rstd[g];
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) { ga[k] = gamma[c + k]; be[k] = beta[c + k]; }
+    for (int k = 0; k < V; ++k) { sc[k] = gamma[c + k] * is[k / E]; sh[k] = beta[c + k]; }
   }
   {
     const Team tm = team_of(w.ng);
@@ -169,8 +174,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
 #pragma unroll
   for (int a = 0; a < A; ++a) {
     const float2 st = stat[group_in_slab(p, l.vx * V + a * E)];
-    c1[a] = st.x;
-    c2[a] = st.y;
+    c1[a] = -st.x * is[a];  // gx = r gamma dz - r c1 - (x - mean) r^2 c2
+    c2[a] = -st.y * is[a] * is[a];
   }
   std::conditional_t<DROP, Mask<V>, NoMask> mask(drop, p, w, c);
   const unsigned long long place = (unsigned long long)l.ry * p.C + c, row_places = (unsigned long long)p.row_lanes * p.C;
@@ -185,11 +190,10 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<D
       if (gy.n > 1) add_more_gy<DT, V, U>(gy, p, w, l, t, u, g);
       if constexpr (DROP) mask.apply(g, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
 #pragma unroll
-      for (int k = 0; k < V; ++k) { f[k] = (f[k] - mu[k / E]) * is[k / E]; z[k] = __builtin_fmaf(f[k], ga[k], be[k]); }
+      for (int k = 0; k < V; ++k) { f[k] -= mu[k / E]; z[k] = __builtin_fmaf(f[k], sc[k], sh[k]); }
       act_bwd<V>(g, z, act);
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        g[k] = is[k / E] * __builtin_fmaf(-f[k], c2[k / E], __builtin_fmaf(ga[k], g[k], -c1[k / E]));
+      for (int k = 0; k < V; ++k) g[k] = __builtin_fmaf(f[k], c2[k / E], __builtin_fmaf(sc[k], g[k], c1[k / E]));
       if (t.valid(u, l.ry)) os.store(o, u, g);
     }
     if (FAR ? t.index + p.last.chunks >= p.tiles : t.index < p.last.chunks) break;

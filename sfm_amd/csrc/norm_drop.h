@@ -137,7 +137,7 @@ template <int V>
 __device__ __forceinline__ void act_bwd(float (&g)[V], const float (&z)[V], int act) {
   if (act == kActElu) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) g[k] = z[k] > 0.0f ? g[k] : g[k] * exp_fast(z[k]);
+    for (int k = 0; k < V; ++k) g[k] *= exp_fast(__builtin_elementwise_minimum(z[k], 0.0f));  // (a NaN stays one)
   } else if (act == kActRelu) {
 #pragma unroll
     for (int k = 0; k < V; ++k) g[k] = z[k] > 0.0f ? g[k] : 0.0f;
