@@ -439,7 +439,7 @@ int sfm_snippet_unpack(const unsigned char* seq, const float* K, int B, int H, i
  * the key `seed`, low half of a word first; it is kept if they are >= threshold, so the probability is threshold / 65536.
  *
  * sfm_dropout: y = keep ? x * 65536 / (65536 - threshold) : 0 for `items` dense items of item_elems elements (rows of C channels),
- * and, applied to dL/dy, its own backward. */
+ * and, applied to dL/dy, its own backward.  SFM_ERR_TOO_LARGE: 2^32 - 256 blocks of eight elements, each item's rounded up. */
 #define SFM_F32 0
 #define SFM_BF16 1
 #define SFM_F16 2

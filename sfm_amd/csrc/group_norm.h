@@ -234,6 +234,7 @@ template <int DT, int V, bool NT = false> struct Stream {  // NT: nontemporal, f
 
 // The mask of a thread's vector in the rows of a tile, u ascending from 0 in every tile.
 template <int V> struct Mask {
+  static constexpr bool kXor3 = V != 8;  // (philox7)
   const Drop& d;
   DropKey key;
   unsigned item;
@@ -241,7 +242,7 @@ template <int V> struct Mask {
   Draw<V> now, next;
   __device__ __forceinline__ Mask(const Drop& drop, const GnPlan& p, const Where& w, int channel)
       : d(drop), key(drop_key(drop)), item(drop.item0 + w.b), pairs(p.pairs) {
-    if (d.per_channel) now = draw<V>(d, key, item, channel);
+    if (d.per_channel) now = draw<V, kXor3>(d, key, item, channel);
   }
   // place: of the vector in row u; step: places between rows u and u + 1
   __device__ __forceinline__ void apply(float (&f)[V], int u, unsigned long long place, unsigned long long step) {
@@ -251,7 +252,7 @@ template <int V> struct Mask {
           if (u & 1) now = next;
           else draw_pair(d, key, item, place, step, now, next);
         } else now = draw<V>(d, key, item, place);
-      } else now = draw<V>(d, key, item, place);
+      } else now = draw<V, kXor3>(d, key, item, place);
     }
     drop_apply<V>(f, now, d);
   }

@@ -171,13 +171,17 @@ __device__ __forceinline__ DropKey drop_key(const Drop& d) {
   return {(unsigned)seed, (unsigned)(seed >> 32), d.rng ? (unsigned)d.rng[1] : d.step};
 }
 
-__device__ __forceinline__ uint4 philox7(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned k0, unsigned k1) {
+// XOR3: a ^ b ^ c as one instruction, two less a round.  Not where eight elements of two 16-bit tensors are in registers with their sums and
+// scales: it takes a few registers more, and those are spilled (backward's sums of 13.6 MB bf16 12.3 -> 15.1 us; elsewhere: dropout alone
+// of 27 MB bf16 12.0 -> 11.5, forward's last pass of 0.5 GB fp32 173 -> 168).
+template <bool XOR3> __device__ __forceinline__ uint4 philox7(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned k0, unsigned k1) {
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
     const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-    c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+    const unsigned hi_a = (unsigned)(a >> 32), hi_b = (unsigned)(b >> 32);
+    c0 = XOR3 ? __builtin_amdgcn_bitop3_b32(hi_b, c1, k0, 0x96) : hi_b ^ c1 ^ k0;
     c1 = (unsigned)b;
-    c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+    c2 = XOR3 ? __builtin_amdgcn_bitop3_b32(hi_a, c3, k1, 0x96) : hi_a ^ c3 ^ k1;
     c3 = (unsigned)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -185,16 +189,16 @@ __device__ __forceinline__ uint4 philox7(unsigned c0, unsigned c1, unsigned c2, 
   return make_uint4(c0, c1, c2, c3);
 }
 
-__device__ __forceinline__ uint4 block_words(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
-  return philox7((unsigned)(place >> 3), item, key.step, d.layer, key.k0, key.k1);
+template <bool XOR3 = true> __device__ __forceinline__ uint4 block_words(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
+  return philox7<XOR3>((unsigned)(place >> 3), item, key.step, d.layer, key.k0, key.k1);
 }
 
 // the 16-bit numbers of elements place .. place + V - 1 of an item, two in a word.  V is a power of two <= 8 that divides place: the V
 // elements lie in one block of eight.
 template <int V> struct Draw { unsigned w[(V + 1) / 2]; };
-template <int V>
+template <int V, bool XOR3 = true>
 __device__ __forceinline__ Draw<V> draw(const Drop& d, const DropKey& key, unsigned item, unsigned long long place) {
-  const uint4 r = block_words(d, key, item, place);
+  const uint4 r = block_words<XOR3>(d, key, item, place);
   Draw<V> o;
   if constexpr (V == 8) { o.w[0] = r.x; o.w[1] = r.y; o.w[2] = r.z; o.w[3] = r.w; }
   else if constexpr (V == 4) { o.w[0] = place & 4 ? r.z : r.x; o.w[1] = place & 4 ? r.w : r.y; }
@@ -226,7 +230,7 @@ __device__ __forceinline__ void drop_apply(float (&f)[V], const Draw<V>& r, cons
   const unsigned t = d.threshold << 16;
 #pragma unroll
   for (int k = 0; k < V; ++k)  // a dropped infinity or NaN is 0 as well
-    f[k] = (k & 1 ? r.w[k / 2] : r.w[k / 2] << 16) >= t ? f[k] * d.scale : 0.0f;
+    f[k] = (k & 1 ? r.w[k / 2] >= t : (unsigned short)r.w[k / 2] >= (unsigned short)d.threshold) ? f[k] * d.scale : 0.0f;
 }
 
 // the same as bits: what a lane hands to others

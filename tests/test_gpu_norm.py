@@ -306,6 +306,46 @@ def test_dropout(dev, shape, per_channel, dtype):
     assert not y.isnan().any()
 
 
+def test_dropout_of_many_blocks(dev):
+    """more workgroups than one dimension of a grid holds, and offsets past 32 bits: an item's result is that of the item by itself"""
+    x = torch.ones(2050, 2 ** 22, dtype=torch.bfloat16, device=dev)
+    mask = lambda first: sfm_amd.DropoutMask(0.5, (3, 4), first_item=first)  # noqa: E731
+    y = sfm_amd.dropout(x, mask(0))
+    for first, last in ((0, 2), (1023, 1025), (2046, 2050)):
+        want = sfm_amd.dropout(x[first:last], mask(first))
+        assert torch.equal(y[first:last], want) and 0.4 < float(want.float().mean()) / 2 < 0.6
+    del y
+    x = torch.ones(3, 2 ** 29 + 1, 3, dtype=torch.float16, device=dev)  # items that start and end in the middle of a block
+    y = sfm_amd.dropout(x, mask(0))
+    assert torch.equal(y[2:], sfm_amd.dropout(x[2:], mask(2)))
+
+
+def test_group_norm_of_many_elements(dev):
+    """offsets past 32 bits: an item's result is that of the item by itself, but for the order of its sums.  Each of the two is off by at most
+    what `compare` allows: together two half steps of bf16 and twice the fp32 part, with the largest factors of the tensor"""
+    g = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randn(3, 1500001, 512, dtype=torch.bfloat16, device=dev, generator=g)
+    gy = torch.randn(x.shape, dtype=torch.bfloat16, device=dev, generator=g)
+    gamma, beta = torch.ones(512, device=dev), torch.zeros(512, device=dev)
+    mask = lambda first: sfm_amd.DropoutMask(0.25, (3, 4), first_item=first)  # noqa: E731
+
+    def run(x, gy, first):
+        x.requires_grad_(True)
+        y = sfm_amd.group_norm_act(x, gamma, beta, 4, dropout=mask(first))
+        return y.detach(), torch.autograd.grad(y, x, gy)[0]
+
+    y, gx = run(x, gy, 0)
+    scale, most, steep = 4 / 3, float(x.detach().abs().max()), float(gy.abs().max())
+    assert 0.99 < float(x.detach()[2].float().var()) < 1.01
+    for k in (0, 2):
+        want_y, want_gx = run(x.detach()[k:k + 1], gy[k:k + 1], k)
+        for at in range(0, x.shape[1], 300001):  # (in pieces: the comparison is in fp32)
+            a, b = y[k, at:at + 300001].float(), want_y[0, at:at + 300001].float()
+            assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() * (1 + 2.0 ** -6) + 80 * U * scale * (2 + 3 * most)).all())
+            a, b = gx[k, at:at + 300001].float(), want_gx[0, at:at + 300001].float()
+            assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() * (1 + 2.0 ** -6) + 320 * U * scale * 1.01 * steep * (1 + 1.01 * most) ** 2).all())
+
+
 def test_dropout_of_what_is_not_finite(dev):
     x = torch.full((4, 64, 8), float("inf"), device=dev)
     x[2:] = float("nan")
