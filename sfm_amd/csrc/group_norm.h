@@ -26,7 +26,8 @@ namespace {
 // kernels' bounds hold their registers down to that): one more than fits is a second round of the whole length.  Measured at 0.5 GB
 // a tensor, us: statistics at 4 / 6 / 8: 97 / 94 / 98; forward's last pass fp32 at 4 / 6: 180 / 171, bf16 at 4 / 6: 193 / 200; backward's sums fp32 at 4 / 5: 194 / 172
 // (16-bit types hold two vectors of eight in registers: 4); its last pass fp32 at 4 / 5: 251 / 245.
-// Vectors of up to four bytes take few registers and have few bytes in flight: more.
+// Vectors of up to four bytes take few registers and have few bytes in flight: more.  (Without and with, us for a step of 8x128x416 rows: 45
+// channels fp32 159 and 144, bf16 151 and 128; 199 bf16 729 and 544.)
 constexpr int waves_stats(int es, int V) { return es * V <= 4 ? 8 : 6; }
 constexpr int waves_apply(int es, int V) { return es * V <= 4 || es == 4 ? 6 : 4; }
 constexpr int waves_sums(int es, int V) { return es * V <= 4 ? 8 : es == 4 ? 5 : 4; }
@@ -35,8 +36,9 @@ constexpr int waves_bwd_apply(int es, int V) { return es * V <= 4 ? 6 : es == 4 
 constexpr int bound_of(int groups_of_vector, int waves) { return groups_of_vector <= 2 ? waves : 4; }
 constexpr int kCUs = 256;
 constexpr int kMaxChunks = 1024;
-// rows a thread has in flight: more of them where a channel count that 16 bytes do not divide makes its vectors shorter
-constexpr int batch_of(int vector_bytes) { return vector_bytes >= 16 ? 4 : 8; }
+// Rows a thread has in flight: more of them where an odd channel count makes its vectors short.  Four and eight, us for a step of 8x128x416
+// rows: 45 channels bf16 134 and 128, 90 bf16 144 and 135; with vectors of eight bytes 100 bf16 148 and 153, 50 fp32 137 and 141.
+constexpr int batch_of(int vector_bytes) { return vector_bytes > 4 ? 4 : 8; }
 
 // How an item is cut: channels into slabs (whole groups, or an even part of one wide group), rows into tiles of U * row_lanes
 // rows (U = batch_of), and the tiles in turn to the chunks (tile t to chunk t % chunks), one workgroup each.  In turn and not in runs: the

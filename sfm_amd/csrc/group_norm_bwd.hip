@@ -24,6 +24,8 @@ __device__ __forceinline__ void add_more_gy(const GySrc& s, const GnPlan& p, con
 }
 
 // ---- backward, first launch: per_group [B][G][P] (sum gamma dz, sum gamma dz xhat), per_channel [C][B][chunks] (sum dz, sum dz xhat)
+// Bound by memory: two tensors of 0.49 GB fp32 in 160 us, 6.1 TB/s; of 0.54 GB bf16 with silu in 202, 5.3 TB/s with the ALUs busy 62 % of it
+// (a tile's loads are asked for when the one before is done; row by row as in the forward's last pass 194, but 180 in fp32 with a mask, which spills).
 template <int DT, int V, int E, bool DROP>
 __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::value, V))) void gn_bwd_sums_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                              const float* __restrict__ gamma, const float* __restrict__ beta,
@@ -114,7 +116,8 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_sums(ElemBytes<DT>::v
 }
 
 // ---- backward, second launch: the first param_blocks workgroups sum the channel partials over items and chunks (a wave per
-// channel), the others write gx
+// channel), the others write gx.  Bound by memory: two tensors of 0.54 GB bf16 read and one written in 270 us, 6.0 TB/s, where the pattern
+// without arithmetic takes 263.
 template <int DT, int V, int E, bool DROP, bool FAR>
 __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_bwd_apply(ElemBytes<DT>::value, V))) void gn_bwd_apply_kernel(const void* __restrict__ x, long long ldx, GySrc gy,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta,
