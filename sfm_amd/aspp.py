@@ -11,6 +11,7 @@ resnet/resnet_utils.py:232-251; csrc/bn_elu.hip), and ``conv2d_bn_elu`` chains t
 from __future__ import annotations
 
 import contextlib
+import operator
 import weakref
 
 import torch
@@ -614,7 +615,7 @@ def _check_level(params, concat, skip_feat, use_skip, use_skip2, skip2, need_mov
         _same_device(concat, *([q["w"]] if nm != "skip_bn" else []), *tensors.values())
         flat += vecs if nm == "skip_bn" else [q["w"], *vecs]
         extras[nm] = {k: q[k] for k in ("moving_mean", "moving_var") if q.get(k) is not None}
-        if groups is not None and (int(groups) < 1 or cv % int(groups)):
+        if groups is not None and (groups < 1 or cv % groups):
             raise ValueError(f"groups must divide the {cv} channels of {nm}, got {groups}")
         if need_moving and len(extras[nm]) != 2:
             raise ValueError(f"is_training=False needs {nm}.moving_mean and {nm}.moving_var")
@@ -709,7 +710,7 @@ def disp_bottleneck_dense(params: dict, concat: Tensor, skip_feat: Tensor = None
     from .pyramid import resize_bilinear
     import functools
     import os
-    groups = None if groups is None else int(groups)
+    groups = None if groups is None else operator.index(groups)
     masks = _level_masks(dropout) if is_training else {}
     if not is_training and groups is None:
         return _dense_level_infer(params, concat, skip_feat, rates, use_skip, use_skip2, skip2)

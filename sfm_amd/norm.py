@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -87,11 +88,11 @@ class DropoutMask:
             self.rng, self.seed, self.step = rng, 0, 0
         else:
             seed, step = rng
-            self.rng, self.seed, self.step = None, int(seed) % 2 ** 64, int(step) % 2 ** 32
+            self.rng, self.seed, self.step = None, operator.index(seed) % 2 ** 64, operator.index(step) % 2 ** 32
         for name, v in (("layer", layer), ("first_item", first_item)):
-            if not 0 <= int(v) < 2 ** 32:
+            if not 0 <= operator.index(v) < 2 ** 32:
                 raise ValueError(f"{name} must be in [0, 2^32), got {v}")
-        self.layer, self.per_channel, self.first_item = int(layer), bool(per_channel), int(first_item)
+        self.layer, self.per_channel, self.first_item = operator.index(layer), bool(per_channel), operator.index(first_item)
 
     @property
     def probability(self) -> float:
@@ -234,7 +235,7 @@ def group_norm_act(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon:
         _check_mask(dropout, x)
         if dropout.threshold == 0:
             dropout = None
-    groups = int(groups)
+    groups = operator.index(groups)
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"groups must divide the {C} channels, got {groups}")
     if torch.is_grad_enabled() and (_sink_of(gamma) is not None or _sink_of(beta) is not None):

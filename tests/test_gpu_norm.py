@@ -543,7 +543,7 @@ def test_gradients_are_born_in_the_buckets(dev):
 
 def test_refusals_with_device_tensors(dev):
     x, g = torch.zeros(2, 3, 8, device=dev), torch.ones(8, device=dev)
-    for kw, err in ((dict(groups=3), ValueError), (dict(groups=0), ValueError), (dict(groups=16), ValueError),
+    for kw, err in ((dict(groups=3), ValueError), (dict(groups=0), ValueError), (dict(groups=16), ValueError), (dict(groups=2.0), TypeError),
                     (dict(groups=2, epsilon=0.0), ValueError), (dict(groups=2, epsilon=float("nan")), ValueError),
                     (dict(groups=2, epsilon=1e-50), ValueError), (dict(groups=2, epsilon=1e39), ValueError),
                     (dict(groups=2, activation="gelu"), ValueError), (dict(groups=2, activation=True), ValueError),

@@ -89,6 +89,12 @@ def test_mask_refuses_values(kw):
         sfm_amd.DropoutMask(**{**dict(p=0.1, rng=(1, 2)), **kw})
 
 
+@pytest.mark.parametrize("kw", [dict(layer=1.0), dict(first_item=0.5), dict(rng=(1.0, 2)), dict(rng=(1, "2"))], ids=str)
+def test_mask_refuses_counters_that_are_no_integers(kw):
+    with pytest.raises(TypeError):
+        sfm_amd.DropoutMask(0.1, **{"rng": (1, 2), **kw})
+
+
 def test_mask_refuses_types_and_takes_the_nearest_probability():
     with pytest.raises(TypeError):
         sfm_amd.DropoutMask(0.1, torch.zeros(2, dtype=torch.int32))
