@@ -17,6 +17,7 @@
 #include <mutex>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/sfm_amd.h"
 
@@ -268,4 +269,7 @@ PYBIND11_MODULE(_autograd, m) {
   m.doc() = "autograd nodes of sfm_amd.norm";
   m.def("group_norm_act", torch::wrap_pybind_function_no_gil(&group_norm_act));
   m.def("dropout", torch::wrap_pybind_function_no_gil(&dropout));
+  m.def("refuse_foreign_leaves", [](const std::string& name, const std::vector<Tensor>& inputs, const Tensor& x) {
+    for (const Tensor& t : inputs) refuse_foreign_leaf(name.c_str(), t, x);
+  });
 }

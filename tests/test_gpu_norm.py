@@ -517,6 +517,15 @@ def test_capture_refuses_leaves_that_an_eager_graph_holds(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, alive) and torch.equal(kept, x.detach() + 1)
+    buckets = sfm_amd.GradBuckets([beta, gamma])  # (the node in Python)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = x.detach() + 1
+            with pytest.raises(RuntimeError, match="stream capture"):
+                sfm_amd.group_norm_act(*leaves, 4)
+    finally:
+        buckets.release()
     del alive
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
