@@ -628,6 +628,9 @@ def _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2, g
         from .norm import _check_mask
         for m in masks.values():
             _check_mask(m, concat)
+    if groups is not None and torch.is_grad_enabled():
+        from .norm import _nodes
+        _nodes().refuse_foreign_leaves("disp_bottleneck_dense", [t for t in (concat, skip_feat, skip2, *flat) if t is not None], concat)
     cfg = (tuple(names), tuple(int(r) for r in rates), bool(use_skip), bool(use_skip2), extras, groups, masks)
     return _DenseLevel.apply(cfg, concat, skip_feat if use_skip else None, skip2 if use_skip2 else None, *flat)
 

@@ -225,3 +225,21 @@ def test_captured_training_steps(dev):
         assert all(torch.equal(a, b) for a, b in zip(got, (*eo, *eg))), k
         seen.append(got[0])
     assert not torch.equal(seen[0], seen[1])
+
+
+def test_capture_refuses_a_level_whose_parameters_an_eager_graph_holds(dev):
+    g = torch.Generator().manual_seed(43)
+    params = on(block(g, 64, 32, True, False), lambda t: t.to(dev).requires_grad_(True))
+    x = on(level_inputs(g, 64, True, False), lambda t: t.to(dev))
+    run = lambda: sfm_amd.disp_bottleneck_dense(params, x["concat"], x["skip_feat"], use_skip2=False, groups=8)[0]  # noqa: E731
+    alive = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = x["concat"] + 1  # (a capture of nothing is warned of)
+        with pytest.raises(RuntimeError, match="stream capture"):
+            run()
+        with torch.no_grad():
+            y = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive) and torch.equal(kept, x["concat"] + 1)
