@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cstdint>
 #include <mutex>
 #include <optional>
 #include <string>
@@ -53,7 +54,9 @@ int dtype_of(const Tensor& x) {
 
 void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
 
-// x [B, ..., C] as rows of C channels ld elements apart: itself if it is dense or a channel slice of a dense buffer, else a copy
+// x [B, ..., C] as rows of C channels ld elements apart: itself if it is dense or a channel slice of a dense buffer, else a copy.  A
+// slice's rows are at least C elements apart in every dimension that has more than one of them: a stride of 0, as expanded tensors
+// and the gradients of sums have, is none (the kernels would read rows that are not there).
 struct Rows {
   Tensor t;
   int64_t ld;
@@ -62,16 +65,20 @@ Rows rows_of(const Tensor& x) {
   const int64_t d = x.dim(), C = x.size(d - 1);
   if (x.is_contiguous()) return {x, C};
   if (C == 1 || x.stride(d - 1) == 1) {
-    int64_t ld = 0, want = 0;
-    bool even = true;
+    int64_t ld = C, want = 0;
+    bool seen = false, even = true;  // seen: a dimension of more than one row has set ld
     for (int64_t k = d - 2; k >= 0 && even; --k) {
       if (x.size(k) == 1) continue;
-      if (ld == 0) ld = want = x.stride(k);
-      even = x.stride(k) == want;
+      if (seen) {
+        even = x.stride(k) == want;
+      } else {
+        seen = true;
+        ld = want = x.stride(k);
+        even = ld >= C && ld <= INT32_MAX / x.element_size();  // (the kernels' limit: rows farther apart are copied)
+      }
       want *= x.size(k);
     }
-    if (even && ld == 0) return {x, C};  // one row
-    if (even && ld >= C) return {x, ld};
+    if (even) return {x, ld};
   }
   return {x.contiguous(), C};
 }
@@ -269,6 +276,11 @@ PYBIND11_MODULE(_autograd, m) {
   m.doc() = "autograd nodes of sfm_amd.norm";
   m.def("group_norm_act", torch::wrap_pybind_function_no_gil(&group_norm_act));
   m.def("dropout", torch::wrap_pybind_function_no_gil(&dropout));
+  // x as rows -> (the tensor itself or a dense copy, elements between rows)
+  m.def("rows_of", [](const Tensor& x) {
+    Rows r = rows_of(x);
+    return pybind11::make_tuple(std::move(r.t), r.ld);
+  });
   m.def("refuse_foreign_leaves", [](const std::string& name, const std::vector<Tensor>& inputs, const Tensor& x) {
     for (const Tensor& t : inputs) refuse_foreign_leaf(name.c_str(), t, x);
   });

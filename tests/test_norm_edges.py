@@ -1,0 +1,76 @@
+"""CPU checks behind tests/test_gpu_norm_edges.py: which layouts the group norm reads in place (nothing here reaches a kernel)."""
+import pytest
+import torch
+
+from sfm_amd import norm
+
+
+def grad_of(f, *shape):
+    """the gradient that autograd hands to y of `shape` from f(y), with the strides it has"""
+    y = torch.randn(*shape, requires_grad=True)
+    seen = []
+    y.register_hook(seen.append)
+    f(y).backward()
+    return seen[0]
+
+
+def _filled(t):
+    """t's strides over a storage of different numbers"""
+    n = t.untyped_storage().nbytes() // t.element_size()
+    return torch.arange(n, dtype=torch.float32).as_strided(t.shape, t.stride(), t.storage_offset())
+
+
+wide = torch.zeros(3, 5, 7, 50)
+LAYOUTS = {  # name -> (tensor, whether it has to be read in place)
+    # broadcast gradients: a stride of 0 in some row dimension
+    "sum over H, W": (grad_of(lambda y: (y.sum(dim=(1, 2)) * torch.randn(4, 32)).sum(), 4, 8, 8, 32), False),
+    "sum over N": (grad_of(lambda y: (y.sum(1) * torch.randn(2, 24)).sum(), 2, 64, 24), False),
+    "sum over W": (grad_of(lambda y: (y.sum(dim=2) * torch.randn(4, 8, 32)).sum(), 4, 8, 8, 32), False),
+    "sum over B": (grad_of(lambda y: (y.sum(0) * torch.randn(8, 32)).sum(), 4, 8, 32), False),
+    "sum over all rows": (grad_of(lambda y: (y.sum(dim=(0, 1, 2)) * torch.randn(32)).sum(), 4, 8, 8, 32), False),
+    "sum over B of [B, C]": (grad_of(lambda y: (y.sum(0) * torch.randn(8)).sum(), 6, 8), False),
+    "sum of one channel": (grad_of(lambda y: y.sum(), 2, 64, 1), False),
+    "sum of everything": (grad_of(lambda y: y.sum(), 2, 9, 24), False),
+    "expanded rows": (torch.zeros(1, 1, 24).expand(4, 10, 24), False),
+    "expanded items": (torch.zeros(1, 10, 24).expand(4, 10, 24), False),
+    "expanded inside": (torch.zeros(4, 10, 1, 24).expand(4, 10, 3, 24), False),
+    "expanded slice": (wide[:, :1, :, 4:28].expand(3, 5, 7, 24), False),
+    # rows that overlap, have gaps of two kinds, or stand in another order
+    "overlapping rows": (torch.zeros(100).as_strided((5, 24), (8, 1)), False),
+    "every second column": (wide[:, :, ::2, 1:25], False),
+    "some rows": (wide[:, 1:4, :, :24], False),
+    "permuted": (wide.permute(0, 2, 1, 3)[..., :24], False),
+    "every second channel": (wide[..., ::2][..., :24], False),
+    # what is read in place
+    "dense": (torch.zeros(3, 5, 24), True),
+    "channel slice": (wide[..., 3:27], True),
+    "one item's slice": (wide[1:2, ..., 3:27], True),
+    "one row": (wide[1:2, 2:3, 3:4, 1:25], True),
+    "one column of one channel": (wide[..., 7:8], True),
+    "no rows": (wide[:0, ..., 1:25], True),
+    "no rows inside": (wide[:, :0, :, 1:25], True),
+}
+
+
+@pytest.mark.parametrize("name", LAYOUTS)
+def test_rows_are_where_the_kernels_look_for_them(name):
+    """the address, the row stride and the reach that the kernels are given lie in the storage and hold the tensor's values"""
+    t, in_place = LAYOUTS[name]
+    x = _filled(t)
+    rows, ld = norm._nodes().rows_of(x)
+    C = x.shape[-1]
+    assert ld >= C
+    n = x.numel() // C
+    if n:
+        have = rows.untyped_storage().nbytes() // rows.element_size()
+        assert rows.storage_offset() + (n - 1) * ld + C <= have, "read past the storage"
+        assert torch.equal(rows.as_strided((n, C), (ld, 1), rows.storage_offset()), x.reshape(n, C))
+    assert (rows is x) == in_place
+
+
+@pytest.mark.parametrize("dtype,ld,in_place", [(torch.float32, 2 ** 29 - 1, True), (torch.float32, 2 ** 29, False), (torch.bfloat16, 2 ** 30 - 1, True),
+                                               (torch.bfloat16, 2 ** 30, False)])
+def test_rows_farther_apart_than_the_kernels_reach_are_copied(dtype, ld, in_place):
+    x = torch.empty(2, 3, ld, dtype=dtype, device="meta")[..., :24]
+    rows, got = norm._nodes().rows_of(x)
+    assert (rows is x) == in_place and got == (ld if in_place else 24)
