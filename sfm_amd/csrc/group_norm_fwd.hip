@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kBlock, bound_of(V / E, waves_apply(ElemBytes<DT>::
       if (more && u < next.steps) raw[u] = xs.row(a, next, u, l.ry);  // as a row has been used, the next tile's is asked for
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
-      act_fwd<V>(f, act);
+      act_fwd<DT, V>(f, act);
       if constexpr (DROP) mask.apply(f, u, (unsigned long long)(t.index * U + u) * row_places + place, row_places);
       if (t.valid(u, l.ry)) ys.store(o, u, f);
     }
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(T) void gn_held_kernel(const void* __restrict__ x, 
       unpack<DT, V>(raw[u], f);
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(f[k] - mu[k / E], sc[k], sh[k]);
-      act_fwd<V>(f, act);
+      act_fwd<DT, V>(f, act);
       if constexpr (DROP) mask.apply(f, u, (unsigned long long)(u * row_lanes + l.ry) * p.C + c, (unsigned long long)row_lanes * p.C);
       store_vec<DT, V>(ys, (long long)u * row_lanes * ldy * kES, f);
     }

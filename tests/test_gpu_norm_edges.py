@@ -1,9 +1,11 @@
 """Group norm and dropout at the edges of what their documentation allows."""
+import numpy as np
 import pytest
 import torch
 
 import sfm_amd
-from test_gpu_norm import inputs
+from oracle import norm_ref as R
+from test_gpu_norm import HALF, TINY, U, f64, inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +46,24 @@ def test_expanded_input(dev, shape, of):
         y = sfm_amd.group_norm_act(*leaves, max(1, shape[-1] // 6))
         runs.append((y, *torch.autograd.grad(y, leaves, gy)))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+# ---- values
+# one launch forward; several chunks of rows; groups wider than a workgroup; an odd channel count
+FORMS = [((2, 100, 32), 4), ((2, 5000, 32), 8), ((2, 19, 4096), 1), ((3, 37, 53, 45), 5)]
+FORM_IDS = ["held", "chunks", "parts", "odd"]
+
+
+@pytest.mark.parametrize("scale", [1e-2, 1e-4, 1e-7])
+@pytest.mark.parametrize("shift", [0.0, 1.0], ids=["beta0", "beta"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("shape,groups", FORMS, ids=FORM_IDS)
+def test_elu_of_small_values(dev, shape, groups, dtype, shift, scale):
+    """with small gamma and beta z is small and as exact, relative to them, as ever; so is elu(z).  z is off by at most 32 roundings of terms
+    no larger than |gamma| (|x| + |x - mean|) / std + |beta| (40 u of that), elu adds 2^-20 of itself in fp32, 2^-16 before a 16-bit rounding"""
+    x, _, gamma, beta = inputs(shape, dtype, 211, dev)
+    gamma, beta = gamma * scale, beta * (scale * shift)
+    want = R.group_norm_act(f64(x), f64(gamma), f64(beta), groups, 1e-5, "elu")
+    size, h = want["z_size"] - 1 + np.abs(f64(beta)), HALF[dtype]
+    bound = 40 * U * size + ((2.0 ** -20 if dtype == torch.float32 else 2.0 ** -16) + h * (1 + 2 * h)) * np.abs(want["y"]) + TINY[dtype]
+    within(sfm_amd.group_norm_act(x, gamma, beta, groups), want["y"], bound, "y")
