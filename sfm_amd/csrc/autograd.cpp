@@ -126,13 +126,15 @@ struct GroupNormActBackward : public torch::autograd::Node {
     }
     const void* gy[1] = {gr.t.data_ptr()};
     const long long ld[1] = {gr.ld};
-    float* at = buf.data_ptr<float>();
+    // a workspace of this pass alone: the node's other passes may be running beside it, as replays of graphs that they were captured into
+    const Tensor ws = at::empty({s.bwd}, gamma.options());
+    const float* at = buf.data_ptr<float>();
     check("sfm_group_norm_act_bwd",
           sfm_group_norm_act_bwd(xr.t.data_ptr(), xr.ld, s.dt, gy, ld, 1, gamma.data_ptr<float>(), beta.data_ptr<float>(), at,
                                  at + s.stats / 2, s.B, s.N, s.C, s.G, s.act, m.state(rng), m.seed, m.step, m.layer, m.item0,
                                  m.threshold, m.per_channel, need_x ? out[0].data_ptr() : nullptr,
                                  need_p ? out[1].data_ptr<float>() : nullptr, need_p ? out[2].data_ptr<float>() : nullptr,
-                                 at + s.stats, stream_of(x)));
+                                 ws.data_ptr<float>(), stream_of(x)));
     return out;
   }
 
@@ -225,8 +227,8 @@ Tensor group_norm_act(const Tensor& x, const Tensor& gamma, const Tensor& beta, 
       TORCH_CHECK_VALUE(s.fwd > 0 && s.bwd > 0, "unsupported group-norm shape ", x.sizes(), " with ", groups, " groups (rc ",
                         std::min(s.fwd, s.bwd), ")");
       s.stats = 2 * s.B * s.G;
-      // one buffer for the statistics and the workspace, of both directions where a backward may come
-      buf = at::empty({grad ? s.stats + std::max(s.fwd, s.bwd) : s.fwd}, gamma.options());
+      // one buffer for the statistics, where a backward may come, and the workspace
+      buf = at::empty({grad ? s.stats + s.fwd : s.fwd}, gamma.options());
       float* at = buf.data_ptr<float>();
       const Rows xr = rows_of(x);
       check("sfm_group_norm_act_fwd",

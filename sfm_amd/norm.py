@@ -128,8 +128,7 @@ def _check_mask(mask, x: Tensor) -> None:
 
 # ----------------------------------------------------------------------------- group norm
 class _Plan:
-    """what is known of a shape: sizes, and the floats of one buffer that holds the statistics (2 B G) and behind them the workspace
-    of either direction"""
+    """what is known of a shape: sizes, and the floats of the statistics (2 B G) and of the workspace of either direction"""
 
     __slots__ = ("B", "N", "C", "G", "dt", "stats", "fwd", "bwd")
 
@@ -157,10 +156,10 @@ def _plan(shape, dtype, groups) -> _Plan:
 
 
 def _raw_gn(plan, x, ld_x, gamma, beta, epsilon, act, mask, y, ld_y, keep):
-    """-> the buffer of statistics and workspace (keep: large enough for the backward, which takes it).  y: a tensor of its own or
-    a channel slice (row stride ld_y)"""
+    """-> the buffer of (keep: the statistics, for the backward, and) the workspace.  y: a tensor of its own or a channel slice (row
+    stride ld_y)"""
     p = plan
-    buf = torch.empty(p.stats + max(p.fwd, p.bwd) if keep else p.fwd, dtype=torch.float32, device=x.device)
+    buf = torch.empty(p.stats + p.fwd if keep else p.fwd, dtype=torch.float32, device=x.device)
     at = buf.data_ptr()
     call("sfm_group_norm_act_fwd", ptr(x), ld_x, p.dt, ptr(gamma), ptr(beta), p.B, p.N, p.C, p.G, epsilon, act, *_ctypes_mask(mask),
          ptr(y), ld_y, at if keep else None, at + 2 * p.stats if keep else None, at + 4 * p.stats if keep else at, stream_of(x))
@@ -168,14 +167,16 @@ def _raw_gn(plan, x, ld_x, gamma, beta, epsilon, act, mask, y, ld_y, keep):
 
 
 def _raw_gn_bwd(plan, x, ld_x, srcs, gamma, beta, buf, act, mask, need_x=True, need_params=True):
-    """srcs: [(tensor whose data pointer is the slice's first channel at row 0, row stride)], summed while loading"""
+    """srcs: [(tensor whose data pointer is the slice's first channel at row 0, row stride)], summed while loading.  buf: the forward's; it is
+    read only, and the workspace is this pass's own: a graph may be run again while a captured pass of it replays"""
     p, n = plan, len(srcs)
+    ws = torch.empty(p.bwd, dtype=torch.float32, device=x.device)
     gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
     gg, gb = (_grad_out(gamma), _grad_out(beta)) if need_params else (None, None)
     at = buf.data_ptr()
     call("sfm_group_norm_act_bwd", ptr(x), ld_x, p.dt, (ctypes.c_void_p * n)(*[t.data_ptr() for t, _ in srcs]),
          (ctypes.c_longlong * n)(*[ld for _, ld in srcs]), n, ptr(gamma), ptr(beta), at, at + 2 * p.stats, p.B, p.N, p.C, p.G, act,
-         *_ctypes_mask(mask), ptr(gx), ptr(gg), ptr(gb), at + 4 * p.stats, stream_of(x))
+         *_ctypes_mask(mask), ptr(gx), ptr(gg), ptr(gb), ptr(ws), stream_of(x))
     return gx, gg, gb
 
 

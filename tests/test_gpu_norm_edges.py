@@ -67,3 +67,29 @@ def test_elu_of_small_values(dev, shape, groups, dtype, shift, scale):
     size, h = want["z_size"] - 1 + np.abs(f64(beta)), HALF[dtype]
     bound = 40 * U * size + ((2.0 ** -20 if dtype == torch.float32 else 2.0 ** -16) + h * (1 + 2 * h)) * np.abs(want["y"]) + TINY[dtype]
     within(sfm_amd.group_norm_act(x, gamma, beta, groups), want["y"], bound, "y")
+
+
+# ---- what is kept and who writes it
+def _saved(f):
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        return f(), kept
+
+
+@pytest.mark.parametrize("buckets", [False, True])
+def test_a_backward_writes_nothing_that_is_kept(dev, buckets):
+    """a graph may be run several times, and its passes captured into graphs of their own that replay side by side: what the node keeps is only
+    read, and each pass has a workspace to itself"""
+    x, gy, gamma, beta = inputs((4, 900, 48), torch.float32, 221, dev)
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    sink = sfm_amd.GradBuckets([beta, gamma]) if buckets else None
+    try:
+        y, kept = _saved(lambda: sfm_amd.group_norm_act(*leaves, 6))
+        before = [t.detach().clone() for t in kept]
+        assert len(kept) == 4
+        first = [g.clone() for g in torch.autograd.grad(y, leaves, gy, retain_graph=True)]
+        assert all(torch.equal(a.view(torch.int32), b.view(torch.int32)) for a, b in zip(kept, before))
+        assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, gy)))
+    finally:
+        if sink:
+            sink.release()
