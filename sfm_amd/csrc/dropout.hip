@@ -132,7 +132,7 @@ extern "C" int sfm_dropout(const void* x, int dtype, long long items, long long 
   if (((uintptr_t)x | (uintptr_t)y) & (es - 1)) return SFM_ERR_ARG;
   const long long blocks = item_elems / 8 + (item_elems % 8 != 0);
   // items and blocks are counted in 32 bits, up to a workgroup past the last
-  if (items > 0xffffffffll - item0 || (__int128)items * blocks > 0xffffffffll - kBlock) return SFM_ERR_TOO_LARGE;
+  if (items > (1ll << 32) - item0 || (__int128)items * blocks > 0xffffffffll - kBlock) return SFM_ERR_TOO_LARGE;
   const unsigned total = (unsigned)(items * blocks), groups = (total + kBlock - 1) / kBlock;
   const bool whole = item_elems % 8 == 0, away = far(2 * items * item_elems * es);
   auto launch = [&](auto dt) {

@@ -229,7 +229,7 @@ extern "C" int sfm_group_norm_act_bwd(const void* x, long long ld_x, int dtype, 
       (!gx && !ggamma) || (gx && !rows_ok(gx, C, C, es)) || (!ggamma != !gbeta) || !ws || ((uintptr_t)ws & 7) || act < kActNone ||
       act > kActSilu || !drop_args(rng, seed, step, layer, item0, threshold, per_channel, d))
     return SFM_ERR_ARG;
-  if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > 0xffffffffll - item0)) return SFM_ERR_TOO_LARGE;
+  if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > (1ll << 32) - item0)) return SFM_ERR_TOO_LARGE;
   GySrc src{};
   src.n = n_gy;
   for (int k = 0; k < n_gy; ++k) {

@@ -342,7 +342,7 @@ extern "C" int sfm_group_norm_act_fwd(const void* x, long long ld_x, int dtype, 
       act < kActNone || act > kActSilu || (!save_mean != !save_rstd) ||
       !drop_args(rng, seed, step, layer, item0, threshold, per_channel, d))
     return SFM_ERR_ARG;
-  if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > 0xffffffffll - item0)) return SFM_ERR_TOO_LARGE;
+  if (threshold && ((__int128)N * C > ((__int128)1 << 35) || B > (1ll << 32) - item0)) return SFM_ERR_TOO_LARGE;
   hipStream_t stream = (hipStream_t)stream_;
   float2* part = reinterpret_cast<float2*>(ws);
   const int held = held_threads(p, es);

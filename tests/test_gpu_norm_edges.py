@@ -93,3 +93,16 @@ def test_a_backward_writes_nothing_that_is_kept(dev, buckets):
     finally:
         if sink:
             sink.release()
+
+
+@pytest.mark.parametrize("per_channel", [False, True])
+def test_last_item_of_the_counter(dev, per_channel):
+    """first_item plus the batch size may be 2^32"""
+    x, gy, gamma, beta = inputs((2, 30, 24), torch.float32, 219, dev)
+    mask = sfm_amd.DropoutMask(0.3, (8, 9), per_channel=per_channel, first_item=2 ** 32 - 2)
+    keep = torch.from_numpy(R.keep_mask((2, 30, 24), mask.threshold, 8, 9, 0, per_channel, 2 ** 32 - 2).copy()).to(dev)
+    plain = sfm_amd.group_norm_act(x, gamma, beta, 4)
+    x.requires_grad_(True)
+    for y, of in ((sfm_amd.dropout(x, mask), x.detach()), (sfm_amd.group_norm_act(x, gamma, beta, 4, dropout=mask), plain)):
+        assert torch.equal(y == 0, ~keep | (of == 0))
+        torch.autograd.grad(y, x, gy)

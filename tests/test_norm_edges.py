@@ -74,3 +74,14 @@ def test_rows_farther_apart_than_the_kernels_reach_are_copied(dtype, ld, in_plac
     x = torch.empty(2, 3, ld, dtype=dtype, device="meta")[..., :24]
     rows, got = norm._nodes().rows_of(x)
     assert (rows is x) == in_place and got == (ld if in_place else 24)
+
+
+@pytest.mark.parametrize("item0,rc", [(2 ** 32 - 1, -2), (2 ** 32 - 2, -1)])
+def test_items_that_the_counter_holds(item0, rc):
+    """two items behind item0: refused where the second would be item 2^32; else the call goes on to the next refusal, its missing tensors"""
+    import ctypes
+    from sfm_amd import _lib
+    lib, f = _lib.load(), 0x10000  # (stands for a device address: nothing is read before the refusal)
+    mask = (None, 0, 0, 0, item0, 9, 0)
+    src, ld = (ctypes.c_void_p * 1)(None if rc == -1 else f), (ctypes.c_longlong * 1)(8)
+    assert lib.sfm_group_norm_act_bwd(f, 8, 0, src, ld, 1, f, f, f, f, 2, 3, 8, 4, 1, *mask, f, f, f, f, None) == rc
