@@ -185,10 +185,10 @@ class _GroupNormActInBuckets(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, plan, epsilon, act, mask):
-        x = x.contiguous()
+        x, ld = _nodes().rows_of(x)  # itself, if it is dense or a channel slice
         with torch.cuda.device(x.device):
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            buf = _raw_gn(plan, x, plan.C, gamma, beta, epsilon, act, mask, y, plan.C, True) if plan.fwd else None
+            buf = _raw_gn(plan, x, ld, gamma, beta, epsilon, act, mask, y, plan.C, True) if plan.fwd else None
         ctx.save_for_backward(x, gamma, beta, buf, None if mask is None else mask.rng)
         ctx.cfg = (plan, act, mask)
         return y
@@ -203,7 +203,8 @@ class _GroupNormActInBuckets(torch.autograd.Function):
             return torch.zeros_like(x), torch.zeros_like(gamma), torch.zeros_like(beta), None, None, None, None
         need_x, need_g, need_b = ctx.needs_input_grad[:3]
         with torch.cuda.device(x.device):
-            return (*_raw_gn_bwd(plan, x, plan.C, ((gy.contiguous(), plan.C),), gamma, beta, buf, act, mask, need_x, need_g or need_b),
+            x, ld = _nodes().rows_of(x)
+            return (*_raw_gn_bwd(plan, x, ld, (_nodes().rows_of(gy),), gamma, beta, buf, act, mask, need_x, need_g or need_b),
                     None, None, None, None)
 
 
