@@ -435,16 +435,17 @@ def _raw_bn_bwd(x, y, ld_y, srcs, q, stats, act):
     return gx, gg, gb
 
 
-def _level_norm(P, groups, masks):
+def _level_norm(P, groups, masks, keep):
     """norm(name, x, act, y, ld_y): the normaliser (and activation, and mask) of the dense x into y, a tensor of its own or a channel
-    slice -> what its backward needs"""
+    slice -> what its backward needs (keep False: none will come, a group norm keeps nothing)"""
     if groups is None:
         return lambda name, x, act, y, ld_y: _raw_bn(x, P[name], act, y, ld_y)
     from . import norm as N
 
     def norm(name, x, act, y, ld_y):
         plan = N._plan(x.shape, x.dtype, groups)
-        return plan, N._raw_gn(plan, x, x.shape[-1], P[name]["gamma"], P[name]["beta"], N.GN_EPSILON, act, masks.get(name), y, ld_y, True)
+        buf = N._raw_gn(plan, x, x.shape[-1], P[name]["gamma"], P[name]["beta"], N.GN_EPSILON, act, masks.get(name), y, ld_y, keep)
+        return (plan, buf) if keep else None
     return norm
 
 
@@ -466,7 +467,7 @@ _LEVEL_CONVS = ("up", "sup", "aspp_up", "aspp_up2", "skip", "skip2", "out")
 class _DenseLevel(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, concat, skip_feat, skip2, *flat):
-        names, rates, use_skip, use_skip2, extras, groups, masks = cfg
+        names, rates, use_skip, use_skip2, extras, groups, masks, keep = cfg
         ctx.set_materialize_grads(False)
         # name -> dict(w, gamma, beta) / dict(gamma, beta) for 'skip_bn', plus the moving statistics (not differentiated)
         P, k = {}, 0
@@ -479,7 +480,7 @@ class _DenseLevel(torch.autograd.Function):
         dims = (B, H, W)
         C = P["sup"]["w"].shape[3]
         nC = (5 if use_skip2 else 4) * C
-        norm = _level_norm(P, groups, masks)
+        norm = _level_norm(P, groups, masks, keep)
         with torch.cuda.device(concat.device):
             u0 = _raw_resize(concat, H, W)                                                      # :454
             a_up = _raw_conv(u0, u0.shape[3], P["up"]["w"], dims, 0)                            # :455
@@ -518,7 +519,7 @@ class _DenseLevel(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_x, g_up):
-        names, rates, use_skip, use_skip2, _, groups, masks = ctx.cfg
+        names, rates, use_skip, use_skip2, _, groups, masks, _ = ctx.cfg
         P, st = ctx.P, ctx.st
         if any(rng._version != v for rng, v in ctx.drawn):
             raise RuntimeError("the (seed, step) tensor of the level's dropout has been modified by an inplace operation since its "
@@ -631,7 +632,8 @@ def _dense_level(params, concat, skip_feat, rates, use_skip, use_skip2, skip2, g
     if groups is not None and torch.is_grad_enabled():
         from .norm import _nodes
         _nodes().refuse_foreign_leaves("disp_bottleneck_dense", [t for t in (concat, skip_feat, skip2, *flat) if t is not None], concat)
-    cfg = (tuple(names), tuple(int(r) for r in rates), bool(use_skip), bool(use_skip2), extras, groups, masks)
+    keep = torch.is_grad_enabled() and any(t.requires_grad for t in (concat, skip_feat, skip2, *flat) if t is not None)
+    cfg = (tuple(names), tuple(int(r) for r in rates), bool(use_skip), bool(use_skip2), extras, groups, masks, keep)
     return _DenseLevel.apply(cfg, concat, skip_feat if use_skip else None, skip2 if use_skip2 else None, *flat)
 
 

@@ -188,7 +188,7 @@ class _GroupNormActInBuckets(torch.autograd.Function):
         x, ld = _nodes().rows_of(x)  # itself, if it is dense or a channel slice
         with torch.cuda.device(x.device):
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            buf = _raw_gn(plan, x, ld, gamma, beta, epsilon, act, mask, y, plan.C, True) if plan.fwd else None
+            buf = _raw_gn(plan, x, ld, gamma, beta, epsilon, act, mask, y, plan.C, any(ctx.needs_input_grad)) if plan.fwd else None
         ctx.save_for_backward(x, gamma, beta, buf, None if mask is None else mask.rng)
         ctx.cfg = (plan, act, mask)
         return y

@@ -6,6 +6,7 @@ import torch
 import sfm_amd
 from oracle import norm_ref as R
 from test_gpu_norm import HALF, TINY, U, f64, inputs, within
+from test_gpu_norm_decoder import block, level_inputs, on
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +137,42 @@ def test_slices_are_read_in_place_with_buckets(dev):
         assert torch.equal(sfm_amd.group_norm_act(z, gamma, beta, 4), sfm_amd.group_norm_act(z.contiguous(), gamma, beta, 4))
     finally:
         sink.release()
+
+
+# ---- in the decoder
+def _level(dev):
+    g = torch.Generator().manual_seed(225)
+    params, ins = block(g, 64, 32, True, True), level_inputs(g, 64, True, True)
+    return on(params, lambda t: t.to(dev).requires_grad_(True)), on(ins, lambda t: t.to(dev))
+
+
+def test_serving_keeps_nothing_for_a_backward(dev, monkeypatch):
+    """statistics are saved where a backward may come, and there alone"""
+    from sfm_amd import norm
+    saved = []
+
+    def spy(name, *args):
+        if name == "sfm_group_norm_act_fwd":
+            saved.append((args[20] is not None, args[21] is not None))
+        return call(name, *args)
+    call = norm.call
+    monkeypatch.setattr(norm, "call", spy)
+    params, ins = _level(dev)
+    run = lambda **kw: sfm_amd.disp_bottleneck_dense(params, ins["concat"], ins["skip_feat"], (2, 4), True, True, ins["skip2"], groups=8, **kw)  # noqa: E731
+
+    def how(**kw):
+        saved.clear()
+        y, up = run(**kw)
+        return y.detach(), set(saved), len(saved)
+    trained, kept, n = how()
+    assert kept == {(True, True)} and n == 8
+    served, kept, n = how(is_training=False)
+    assert kept == {(False, False)} and n == 8 and torch.equal(served, trained)
+    with torch.no_grad():
+        assert how()[1] == {(False, False)}
+    for q in params.values():
+        for t in q.values():
+            t.requires_grad_(False)
+    assert how()[1] == {(False, False)}       # no leaf wants a gradient
+    ins["skip2"].requires_grad_(True)
+    assert how()[1] == {(True, True)}
