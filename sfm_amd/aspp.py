@@ -511,7 +511,7 @@ class _DenseLevel(torch.autograd.Function):
             xconcat = torch.empty_like(a_out)
             st["out"] = norm("out", a_out, 0, xconcat, C)
         ctx.cfg, ctx.P, ctx.st = cfg, P, st
-        ctx.drawn = [(m.rng, m.rng._version) for m in masks.values() if m.rng is not None]
+        ctx.drawn = [(m.rng, m.rng._version) for m in masks.values() if m.rng is not None] if keep else []
         ctx.acts = (u0, a_up, a_sup, a_au, a_au2, sk, a_sk, s2, a_s2, X, a_out)
         ctx.io = (concat.shape, skip2.shape if use_skip2 else None)
         ctx.save_for_backward(xconcat, upnet, *([skip_feat] if use_skip else []))

@@ -176,3 +176,13 @@ def test_serving_keeps_nothing_for_a_backward(dev, monkeypatch):
     assert how()[1] == {(False, False)}       # no leaf wants a gradient
     ins["skip2"].requires_grad_(True)
     assert how()[1] == {(True, True)}
+
+
+def test_level_draws_under_inference_mode(dev):
+    """a tensor made under inference_mode has no version to check, and no backward that would need it"""
+    params, ins = _level(dev)
+    run = lambda rng: sfm_amd.disp_bottleneck_dense(params, ins["concat"], ins["skip_feat"], (2, 4), True, True, ins["skip2"], groups=8,  # noqa: E731
+                                                    dropout=sfm_amd.DropoutMask(0.2, rng))[0]
+    want = run((5, 6)).detach()
+    with torch.inference_mode():
+        assert torch.equal(run(torch.tensor([5, 6], device=dev)), want)
