@@ -6,12 +6,14 @@
 // stays in the C ABI (include/sfm_amd.h), which this file only calls.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cstdint>
@@ -41,6 +43,14 @@ void check(const char* name, int rc) {
 
 void refuse_second_order(const char* name) {  // a backward runs with gradients on under create_graph=True alone
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its backward was called with create_graph=True");
+}
+
+// These nodes are no operators of torch's dispatcher: a tracer would record nothing of them but the allocation of their results, and
+// its program would return memory as it found it.
+void refuse_tracing(const char* name) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+              name, " cannot be traced (torch.jit.trace, torch.fx): its kernels would not be in the traced program");
 }
 
 int dtype_of(const Tensor& x) {
@@ -109,6 +119,7 @@ struct GroupNormActBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(lock_);
     refuse_second_order("group_norm_act");
+    refuse_tracing("group_norm_act");
     variable_list out(3);
     const Tensor x = x_.unpack(), gamma = gamma_.unpack(), beta = beta_.unpack();
     if (!grads[0].defined()) return out;
@@ -170,6 +181,7 @@ Tensor run_dropout(const Tensor& x_, const Mask& m, const Tensor& rng) {
 variable_list DropoutBackward::apply(variable_list&& grads) {
   std::lock_guard<std::mutex> lock(lock_);
   refuse_second_order("dropout");
+  refuse_tracing("dropout");
   const Tensor rng = m.rng.has_value() ? rng_.unpack() : Tensor();
   if (!grads[0].defined()) return {Tensor()};
   return {run_dropout(grads[0], m, rng)};
@@ -203,6 +215,7 @@ template <typename NodeT, typename... T> std::shared_ptr<NodeT> make_node(const 
 Tensor group_norm_act(const Tensor& x, const Tensor& gamma, const Tensor& beta, int64_t groups, double epsilon, int act,
                       std::optional<Tensor> rng, uint64_t seed, uint32_t step, uint32_t layer, uint32_t item0, int threshold,
                       bool per_channel) {
+  refuse_tracing("group_norm_act");
   Shape s{};
   s.dt = dtype_of(x);
   s.act = act;
@@ -254,6 +267,7 @@ Tensor group_norm_act(const Tensor& x, const Tensor& gamma, const Tensor& beta, 
 
 Tensor dropout(const Tensor& x, std::optional<Tensor> rng, uint64_t seed, uint32_t step, uint32_t layer, uint32_t item0, int threshold,
                bool per_channel) {
+  refuse_tracing("dropout");
   Mask m{std::move(rng), seed, step, layer, item0, threshold, per_channel};
   refuse_forward_mode("dropout", x);
   const bool grad = at::GradMode::is_enabled() && x.requires_grad();
@@ -283,6 +297,7 @@ PYBIND11_MODULE(_autograd, m) {
     Rows r = rows_of(x);
     return pybind11::make_tuple(std::move(r.t), r.ld);
   });
+  m.def("refuse_tracing", [](const std::string& name) { refuse_tracing(name.c_str()); });
   m.def("refuse_foreign_leaves", [](const std::string& name, const std::vector<Tensor>& inputs, const Tensor& x) {
     for (const Tensor& t : inputs) refuse_foreign_leaf(name.c_str(), t, x);
   });

@@ -241,6 +241,7 @@ def group_norm_act(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon:
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"groups must divide the {C} channels, got {groups}")
     if torch.is_grad_enabled() and (_sink_of(gamma) is not None or _sink_of(beta) is not None):
+        _nodes().refuse_tracing("group_norm_act")
         _nodes().refuse_foreign_leaves("group_norm_act", [x, gamma, beta], x)
         return _GroupNormActInBuckets.apply(x, gamma, beta, _plan(shape, x.dtype, groups), epsilon, act, dropout)
     return _nodes().group_norm_act(x, gamma, beta, groups, epsilon, act, *(_NO_MASK if dropout is None else dropout._args()))

@@ -85,3 +85,23 @@ def test_items_that_the_counter_holds(item0, rc):
     mask = (None, 0, 0, 0, item0, 9, 0)
     src, ld = (ctypes.c_void_p * 1)(None if rc == -1 else f), (ctypes.c_longlong * 1)(8)
     assert lib.sfm_group_norm_act_bwd(f, 8, 0, src, ld, 1, f, f, f, f, 2, 3, 8, 4, 1, *mask, f, f, f, f, None) == rc
+
+
+def _node_calls():
+    n, g = norm._nodes(), torch.ones(8)
+    none = (None, 0, 0, 0, 0, 0, False)
+    return {"group_norm_act": lambda x: n.group_norm_act(x, g, g, 2, 1e-5, 1, *none), "dropout": lambda x: n.dropout(x, None, 1, 2, 0, 0, 9, False),
+            "group_norm_act (buckets)": lambda x: n.refuse_tracing("group_norm_act") or x * 1}
+
+
+@pytest.mark.parametrize("name", _node_calls())
+def test_tracing_is_refused(name):
+    """a tracer would record the allocation of the result and nothing of what fills it (refused before a tensor's memory is looked at)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x = _node_calls()[name], torch.zeros(2, 3, 8)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(f, (x,))
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(f)(x)
+    if "buckets" in name:
+        f(x)
