@@ -5,7 +5,7 @@ import torch
 
 import sfm_amd
 from oracle import norm_ref as R
-from test_gpu_norm import HALF, TINY, U, f64, inputs, within
+from test_gpu_norm import HALF, TINY, U, compare, f64, inputs, within
 from test_gpu_norm_decoder import block, level_inputs, on
 
 pytestmark = pytest.mark.gpu
@@ -186,3 +186,74 @@ def test_level_draws_under_inference_mode(dev):
     want = run((5, 6)).detach()
     with torch.inference_mode():
         assert torch.equal(run(torch.tensor([5, 6], device=dev)), want)
+
+
+@pytest.mark.parametrize("first_row", [None, -3.0e4], ids=["no outlier", "outlier"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape,groups", FORMS, ids=FORM_IDS)
+def test_gradients_where_the_mean_is_far_from_the_deviation(dev, shape, groups, dtype, first_row):
+    """mean 1000, deviation about 1 (in fp32 a sum of squares less the squared mean leaves nothing of it), or with a first row far off.
+    y as in `compare`.  d bounds what z and xhat are off by, the mean's rounding being most of it; then act' is off by d, c1 by d and c2 by
+    d (1 + |xhat|) of their largest term, so gx is off by 2 d r s |gamma gy| (1 + |xhat|)^2 beside `compare`'s bound"""
+    x, gy, gamma, beta = inputs(shape, torch.float32, 213, dev)
+    x = x + 1000.0
+    if first_row is not None:
+        x[:, 0] = first_row
+    x, gy = x.to(dtype), gy.to(dtype)
+    want = R.group_norm_act(f64(x), f64(gamma), f64(beta), groups, 1e-5, "elu", f64(gy))
+    d = 40 * U * (1 + want["z_size"].max())
+    extra = 2 * d * want["rstd"].max() * np.abs(f64(gamma)).max() * np.abs(f64(gy)).max() * (1 + want["xhat_max"]) ** 2
+    leaves = [t.requires_grad_(True) for t in (x, gamma, beta)]
+    y = sfm_amd.group_norm_act(*leaves, groups)
+    compare(y, torch.autograd.grad(y, leaves, gy), want, dtype, loose=(extra, 0.0, 0.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape,groups", [((300, 1801, 32), 8), ((300, 1825, 32), 16), ((600, 700, 10), 5), ((500, 613, 36), 9), ((2, 100, 32), 4),
+                                          ((2, 19, 4096), 1), ((3, 37, 53, 90), 5), ((1, 1, 8), 2), ((2, 5000, 32), 4)], ids=str)
+def test_no_row_is_lost_or_counted_twice(dev, shape, groups, dtype):
+    """whole numbers: gbeta = sum gy exactly.  x = +-1 by turns in every group: mean 0, variance 1, ggamma = r sum x gy.  There x - mean, r, the sums'
+    product with it and the result are rounded: 8 u of sum |gy|, which is under half a row's share"""
+    g = torch.Generator().manual_seed(215)
+    C = shape[-1]
+    gy = torch.randint(-1, 2, shape, generator=g).to(dtype).to(dev)
+    x = (1.0 - 2.0 * (torch.arange(C) % 2)).expand(shape).contiguous().to(dtype).to(dev)
+    gamma, beta = (1 + 0.2 * torch.randn(C, generator=g)).to(dev).requires_grad_(True), torch.zeros(C, device=dev, requires_grad=True)
+    gg, gb = torch.autograd.grad(sfm_amd.group_norm_act(x, gamma, beta, groups, activation=None), (gamma, beta), gy)
+    flat = f64(gy).reshape(-1, C)
+    assert np.array_equal(f64(gb), flat.sum(axis=0))
+    bound = 8 * U * np.abs(flat).sum(axis=0)
+    assert bound.max() < 0.5
+    within(gg, (flat * f64(x).reshape(-1, C)).sum(axis=0) / (1 + 1e-5) ** 0.5, bound, "ggamma")
+
+
+@pytest.mark.parametrize("act", ["elu", "silu", "relu", None])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N", [40, 3001])
+def test_gradients_of_what_is_not_finite_stay_in_their_group(dev, N, dtype, act):
+    x, gy, gamma, beta = inputs((3, N, 24), dtype, 217, dev)
+
+    def run(x, gy, mask=None):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, gamma, beta)]
+        y = sfm_amd.group_norm_act(*leaves, 4, activation=act, dropout=mask)
+        return torch.autograd.grad(y, leaves, gy)
+    clean = run(x, gy)
+    hit, chan = torch.zeros(x.shape, dtype=torch.bool, device=dev), torch.zeros(24, dtype=torch.bool, device=dev)
+    hit[1, :, 6:12] = hit[2, :, 18:24] = chan[6:12] = chan[18:24] = True
+    for what in ("x", "gy"):
+        bad = {"x": x.clone(), "gy": gy.clone()}
+        bad[what][1, N - 3, 8] = float("nan")
+        bad[what][2, 3, 23] = float("inf")
+        if act == "relu" and what == "gy":  # (relu' = 0 there would make it 0, or a NaN of inf * 0: not asked for)
+            continue
+        gx, gg, gb = run(bad["x"], bad["gy"])
+        # a mean that is none makes all NaN; with an infinite gy c1 and c2 are infinite, and -c1 - xhat c2 is that or a NaN
+        assert not torch.isfinite(gx[hit]).any() and (what == "gy" or torch.isnan(gx[hit]).all()) and torch.equal(gx[~hit], clean[0][~hit]), what
+        if what == "x":
+            assert torch.isnan(gg[chan]).all()
+        assert torch.equal(gg[~chan], clean[1][~chan]) and torch.equal(gb[~chan], clean[2][~chan]), what
+    # a gradient that the mask drops counts for nothing, whatever it is
+    mask = sfm_amd.DropoutMask(0.5, (6, 7))
+    keep = torch.from_numpy(R.keep_mask(tuple(x.shape), mask.threshold, 6, 7).copy()).to(dev)
+    bad = torch.where(keep, gy, torch.full_like(gy, float("nan")))
+    assert all(torch.equal(a, b) for a, b in zip(run(x, bad, mask), run(x, gy, mask)))

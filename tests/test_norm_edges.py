@@ -105,3 +105,22 @@ def test_tracing_is_refused(name):
         make_fx(f)(x)
     if "buckets" in name:
         f(x)
+
+
+def test_the_bounds_see_a_difference_of_large_sums():
+    """what tests/test_gpu_norm_edges.py allows where the mean is far from the deviation is not enough for a variance that is E[x^2] - mean^2 in
+    fp32, and is enough for one from deviations"""
+    import numpy as np
+    from oracle import norm_ref as R
+    from test_gpu_norm import U, f64, inputs
+    x, _, gamma, beta = inputs((2, 5000, 32), torch.float32, 213, "cpu")
+    x = x + 1000.0
+    want = R.group_norm_act(f64(x), f64(gamma), f64(beta), 8, 1e-5, "elu")
+    v = x.reshape(2, 5000, 8, 4)
+    mean = v.mean(dim=(1, 3), keepdim=True)
+    share = []
+    for var in ((v * v).mean(dim=(1, 3), keepdim=True) - mean * mean, ((v - mean) ** 2).mean(dim=(1, 3), keepdim=True)):
+        y = torch.nn.functional.elu(((v - mean) / (var + 1e-5).sqrt()).reshape(x.shape) * gamma + beta)
+        off = np.abs(f64(y) - want["y"]) / (40 * U * want["z_size"] + U * np.abs(want["y"]))
+        share.append(off[np.isfinite(off)].max() if np.isfinite(off).any() else np.inf)
+    assert share[0] > 10 and share[1] < 1, share
