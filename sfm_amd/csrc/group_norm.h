@@ -23,7 +23,9 @@ namespace {
 
 
 // Workgroups per CU that a pass is launched with; a workgroup is one wave per SIMD, and all of a launch have to be resident (the
-// kernels' bounds hold their registers down to that): one more than fits is a second round of the whole length.  Measured at 0.5 GB
+// kernels' bounds hold their registers down to that): one more than fits is a second round of the whole length.  Some masked kernels
+// of the backward meet their bound with scratch: 8-48 bytes in the sums (16 bits with one or two channels of a group in a vector, and fp32
+// by single elements), 80-84 in the last pass of 16 bits in eights with one, 20 in that of vectors of four.  Measured without a mask, at 0.5 GB
 // a tensor, us: statistics at 4 / 6 / 8: 97 / 94 / 98; forward's last pass fp32 at 4 / 6: 180 / 171, bf16 at 4 / 6: 193 / 200; backward's sums fp32 at 4 / 5: 194 / 172
 // (16-bit types hold two vectors of eight in registers: 4); its last pass fp32 at 4 / 5: 251 / 245.
 // Vectors of up to four bytes take few registers and have few bytes in flight: more.  (Without and with, us for a step of 8x128x416 rows: 45
