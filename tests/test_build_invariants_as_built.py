@@ -55,3 +55,11 @@ def test_group_norm_and_dropout(tmp_path):
                 allowed = SCRATCH.get((which, dt, v, e), SCRATCH.get((which, dt, v, 0), 0))
             assert priv <= allowed, f"{name}: {priv} bytes of scratch, {spill} spilled VGPRs"
     assert count
+
+
+def test_build_compiles_whatever_is_there(monkeypatch):
+    import __graft_entry__ as g
+    ran = []
+    monkeypatch.setattr(g.subprocess, "check_call", lambda args, **kw: ran.append(args))
+    g.build()
+    assert len(ran) == 1 and ran[0][0] == "make" and "-B" in ran[0]
