@@ -429,8 +429,9 @@ int sfm_snippet_unpack(const unsigned char* seq, const float* K, int B, int H, i
  * read at call time) -> gx [B, N, C] dense (may be NULL), ggamma and gbeta [C] (both or neither), summed over items and rows.
  * It reads x and not y, and takes the mask's arguments of the forward.
  * ws: sfm_group_norm_workspace_floats(B, N, C, G, dtype, backward != 0) floats, 8-byte aligned, undefined between calls.
- * Sums are joined in a fixed order: results are bitwise reproducible.  SFM_ERR_TOO_LARGE: more than 2^22 workgroups (an item takes at
- * least one for every 128 bytes of a row), more than 2^40 rows, row strides of 2 GiB; with a mask items of 2^35 elements.
+ * Sums are joined in a fixed order: results are bitwise reproducible.  SFM_ERR_TOO_LARGE: more than 2^22 workgroups (an item takes up to
+ * one for every 128 bytes of a row) or more than 65535 of one row, more than 2^40 rows, row strides of 2 GiB; with a mask items of
+ * 2^35 elements, or items past item 2^32 - 1.
  *
  * The mask (threshold = 0: none) is a function of counters and never stored.  (seed, step): two 64-bit words at `rng` in device
  * memory, read by the kernels (so a replayed graph follows them), or the two arguments if rng is NULL; of step the low 32 bits

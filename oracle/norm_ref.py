@@ -1,5 +1,5 @@
 """Group norm with an activation and counter-based dropout from their definitions, in float64 on the CPU (NumPy): what the kernels
-of sfm_amd/csrc/group_norm.hip and dropout.hip are compared with.  No counterpart in the reference."""
+of sfm_amd/csrc/group_norm_fwd.hip, group_norm_bwd.hip and dropout.hip are compared with.  No counterpart in the reference."""
 import numpy as np
 
 M0, M1, W0, W1 = 0xD2511F53, 0xCD9E8D57, 0x9E3779B9, 0xBB67AE85
